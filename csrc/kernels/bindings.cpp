@@ -57,6 +57,26 @@ void qkv_decode_finish(torch::Tensor acc, torch::Tensor qkv, torch::Tensor k_cac
                        torch::Tensor pos, torch::Tensor cos_t, torch::Tensor sin_t, int64_t H, double eps);
 void gemm_skinny_acc(torch::Tensor w, torch::Tensor x, torch::Tensor acc, int64_t splits);
 void set_pdl(bool on);
+void rotate(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor pos, torch::Tensor cos_t,
+            torch::Tensor sin_t, bool interleaved, bool back, torch::Tensor q_out, c10::optional<torch::Tensor> k_out);
+void paged_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, torch::Tensor v_pages,
+                  torch::Tensor table, torch::Tensor lens, torch::Tensor row_slot, torch::Tensor row_back,
+                  c10::optional<torch::Tensor> cos_t, c10::optional<torch::Tensor> sin_t, bool interleaved, double eps,
+                  bool norm, torch::Tensor q_out);
+void pages_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
+                torch::Tensor parents, torch::Tensor children, torch::Tensor table_out, torch::Tensor lens_out,
+                torch::Tensor refs_out);
+void pages_grow(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor add, int64_t page,
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out);
+void pages_free(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor seqs,
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out);
+void pages_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
+                   torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out);
+void pages_copy(torch::Tensor k, torch::Tensor v, torch::Tensor src, torch::Tensor dst);
+void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
+                     torch::Tensor items, torch::Tensor slot_of_seq, torch::Tensor row_slot, torch::Tensor row_back,
+                     torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot, double scale,
+                     torch::Tensor out, c10::optional<torch::Tensor> lse);
 torch::Tensor gemm_trace();
 }  // namespace nk
 
@@ -101,5 +121,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv_decode_finish", &nk::qkv_decode_finish);
   m.def("gemm_skinny_acc", &nk::gemm_skinny_acc);
   m.def("gemm_trace", &nk::gemm_trace, "MMA-warp wait accounting of the last traced GEMM (measurement)");
+  m.def("rotate", &nk::rotate);
+  m.def("paged_append", &nk::paged_append);
+  m.def("pages_fork", &nk::pages_fork);
+  m.def("pages_grow", &nk::pages_grow);
+  m.def("pages_free", &nk::pages_free);
+  m.def("pages_compact", &nk::pages_compact);
+  m.def("pages_copy", &nk::pages_copy);
+  m.def("paged_attention", &nk::paged_attention);
   m.def("set_pdl", &nk::set_pdl, "programmatic dependent launch for the decode-chain kernels");
 }

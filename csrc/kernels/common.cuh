@@ -17,7 +17,8 @@ constexpr uint32_t kSpinLimit = 1u << 26;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 
 enum : int { kErrNone = 0, kErrTimeoutProducer = 1, kErrTimeoutMma = 2, kErrTimeoutEpilogue = 3,
-             kErrTimeoutOther = 4, kErrBounds = 5 };
+             kErrTimeoutOther = 4, kErrBounds = 5,
+             kErrNoPages = 6 };
 
 // Tile-index checks of the debug build (compiled with -DNANOGPT_DEBUG_BOUNDS,
 // the `_C_bounds` extension): NK_IN_BOUNDS(cond, err) records kErrBounds in

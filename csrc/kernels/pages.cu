@@ -1,0 +1,495 @@
+// Pages of a KV cache: forking sequences (copy of the last, partly filled page),
+// making room for new tokens, freeing sequences, compacting the pool, and plain
+// page copies. All state lives on the device and no call reads it back, so the
+// operators can be queued (or captured in a CUDA graph) without a host wait.
+//
+//   k, v    (layers, pages, kv heads, rows of a page, head dim)
+//   table   (slots, width) int32: a sequence's pages in order, -1 past the last
+//   lens    (slots) int32: tokens of a sequence (0: the slot is empty)
+//   refs    (pages) int32: table entries that name the page (0: the page is free)
+//
+// Full pages are shared between forks and never written again; a partly filled
+// page belongs to one sequence. New pages are the lowest free ones, handed out in
+// the order of the call's list, so every result is defined exactly.
+//
+// Each operator is one launch of a single cluster that rewrites table, lens and
+// refs (into fresh tensors or in place) in phases separated by cluster barriers,
+// and, where rows move, a second launch that copies them from a list of pairs
+// that the first one left in the workspace.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <climits>
+
+#include "common.cuh"
+#include "message.h"
+#include "status.h"
+
+namespace nk {
+namespace {
+
+constexpr int kMetaCtas = 8;        // one portable cluster
+constexpr int kMetaThreads = 1024;
+constexpr int kMetaAll = kMetaCtas * kMetaThreads;
+
+struct PageState {
+  const int *table_in, *lens_in, *refs_in;
+  int *table, *lens, *refs;
+  int slots, width, pages, page;  // page: rows of one
+  int* err;
+};
+
+// Workspace of the metadata kernels (int32): per-CTA counts and totals, then the
+// lists. kListAt is where the first list starts.
+constexpr int kWsCounts = 0, kWsPairs = 8, kListAt = 16;
+
+__device__ __forceinline__ void report(int* err, int code) { atomicCAS(err, 0, code); }
+
+__device__ __forceinline__ bool copies(const PageState& s) { return s.table != s.table_in; }
+
+// table, lens and refs into the outputs, all threads of the cluster.
+__device__ __forceinline__ void copy_state(const PageState& s, int gid) {
+  if (!copies(s)) return;
+  for (long i = gid; i < long(s.slots) * s.width; i += kMetaAll) s.table[i] = s.table_in[i];
+  for (int i = gid; i < s.slots; i += kMetaAll) s.lens[i] = s.lens_in[i];
+  for (int i = gid; i < s.pages; i += kMetaAll) s.refs[i] = s.refs_in[i];
+}
+
+// Exclusive sum over a CTA's threads; every thread also gets the total.
+__device__ __forceinline__ int cta_scan(int v, int* sm, int& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // sm may still be read from an earlier call
+  if (lane == 31) sm[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = sm[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    sm[lane] = w;
+  }
+  __syncthreads();
+  total = sm[31];
+  return (warp ? sm[warp - 1] : 0) + x - v;
+}
+
+// Thread `gid` of the cluster owns pages [lo, hi). Returns how many pages before
+// lo have refs > 0, and the number of all such pages. One cluster barrier.
+__device__ __forceinline__ int live_before(const int* refs, int pages, int gid, int* sm, int* ws, int& lo, int& hi,
+                                           int& live) {
+  const int span = (pages + kMetaAll - 1) / kMetaAll;
+  lo = min(pages, gid * span);
+  hi = min(pages, lo + span);
+  int mine = 0;
+  for (int p = lo; p < hi; ++p) mine += refs[p] > 0;
+  int total;
+  int before = cta_scan(mine, sm, total);
+  const int cta = int(cluster_rank());
+  if (threadIdx.x == 0) ws[kWsCounts + cta] = total;
+  cluster_sync();
+  live = 0;
+  for (int c = 0; c < kMetaCtas; ++c) {
+    const int n = __ldcg(ws + kWsCounts + c);
+    if (c < cta) before += n;
+    live += n;
+  }
+  return before;
+}
+
+__device__ __forceinline__ int meta_gid() { return int(cluster_rank()) * kMetaThreads + int(threadIdx.x); }
+
+// Sequences are handed to the cluster's warps in turn.
+constexpr int kMetaWarps = kMetaAll / 32;
+__device__ __forceinline__ int meta_warp() { return meta_gid() / 32; }
+
+// ---- fork ----------------------------------------------------------------------
+
+// ws lists: owner (slots); then n each of: free pages, pair sources, pair
+// targets, pair rows, lengths of the children to make (-1: none).
+__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+    fork_meta_kernel(const PageState s, const int* __restrict__ parents, const int* __restrict__ children, int n,
+                     int* ws) {
+  __shared__ int sm[32];
+  const int gid = meta_gid();
+  int *owner = ws + kListAt, *spare = owner + s.slots, *src = spare + n, *dst = src + n, *rows = dst + n,
+      *length = rows + n;
+  copy_state(s, gid);
+  for (int i = gid; i < s.slots; i += kMetaAll) owner[i] = INT_MAX;
+  int lo, hi, live;
+  const int before = live_before(s.refs_in, s.pages, gid, sm, ws, lo, hi, live);
+  for (int p = lo, f = lo - before; p < hi && f < n; ++p)
+    if (s.refs_in[p] <= 0) spare[f++] = p;
+  // A slot that the list names twice goes to its first mention.
+  for (int i = gid; i < n; i += kMetaAll) {
+    const int c = children[i];
+    if (c >= 0 && c < s.slots) atomicMin(owner + c, i);
+  }
+  cluster_sync();
+  if (cluster_rank() == 0) {
+    // Which children are made, and the page of each that needs one: by one CTA,
+    // in the list's order.
+    const int span = (n + kMetaThreads - 1) / kMetaThreads;
+    const int i0 = min(n, int(threadIdx.x) * span), i1 = min(n, i0 + span);
+    int mine = 0, total;
+    for (int i = i0; i < i1; ++i) {
+      const int p = parents[i], c = children[i];
+      const bool ok = p >= 0 && p < s.slots && c >= 0 && c < s.slots && __ldcg(owner + c) == i && s.lens_in[c] == 0 &&
+                      s.lens_in[p] >= 0 && s.lens_in[p] <= s.width * s.page;
+      if (!ok) report(s.err, kErrBounds);
+      length[i] = ok ? s.lens_in[p] : -1;
+      mine += ok && length[i] % s.page;
+    }
+    int rank = cta_scan(mine, sm, total);
+    for (int i = i0; i < i1; ++i) {
+      const int len = length[i];
+      const bool part = len >= 0 && len % s.page;
+      src[i] = dst[i] = -1;
+      rows[i] = 0;
+      if (part && rank++ < s.pages - live) {
+        src[i] = s.table_in[long(parents[i]) * s.width + len / s.page];
+        dst[i] = __ldcg(spare + rank - 1);
+        rows[i] = len % s.page;
+      } else if (part) {
+        report(s.err, kErrNoPages);
+        length[i] = -1;
+      }
+    }
+  }
+  cluster_sync();
+  for (int i = meta_warp(); i < n; i += kMetaWarps) {
+    const int len = __ldcg(length + i), lane = threadIdx.x % 32;
+    if (len < 0) continue;
+    const int* from = s.table_in + long(parents[i]) * s.width;
+    int* to = s.table + long(children[i]) * s.width;
+    for (int e = lane; e < len / s.page; e += 32) {
+      const int q = from[e];
+      to[e] = q;
+      if (q >= 0 && q < s.pages) atomicAdd(s.refs + q, 1);
+    }
+    if (lane == 0) {
+      s.lens[children[i]] = len;
+      if (len % s.page) {
+        const int q = __ldcg(dst + i);
+        to[len / s.page] = q;
+        s.refs[q] = 1;
+      }
+    }
+  }
+}
+
+// ---- grow ----------------------------------------------------------------------
+
+// ws list: free pages (pages).
+__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+    grow_meta_kernel(const PageState s, const int* __restrict__ add, int* ws) {
+  __shared__ int sm[32];
+  const int gid = meta_gid();
+  int* spare = ws + kListAt;
+  copy_state(s, gid);
+  int lo, hi, live;
+  const int before = live_before(s.refs_in, s.pages, gid, sm, ws, lo, hi, live);
+  for (int p = lo, f = lo - before; p < hi; ++p)
+    if (s.refs_in[p] <= 0) spare[f++] = p;
+  cluster_sync();
+  if (cluster_rank() != 0) return;
+  const int span = (s.slots + kMetaThreads - 1) / kMetaThreads;
+  const int i0 = min(s.slots, int(threadIdx.x) * span), i1 = min(s.slots, i0 + span);
+  auto need = [&](int i, int& len, int& have) {  // pages that slot i lacks; -1: it cannot be grown
+    const int more = add[i];
+    len = s.lens_in[i];
+    have = (len + s.page - 1) / s.page;
+    if (more < 0 || len < 0 || long(len) + more > long(s.width) * s.page) return -1;
+    return (len + more + s.page - 1) / s.page - have;
+  };
+  int mine = 0, total, len, have;
+  for (int i = i0; i < i1; ++i) mine += max(0, need(i, len, have));
+  int rank = cta_scan(mine, sm, total);
+  for (int i = i0; i < i1; ++i) {
+    const int m = need(i, len, have);
+    if (m < 0) {
+      report(s.err, kErrBounds);
+    } else if (rank + m > s.pages - live) {
+      report(s.err, kErrNoPages);  // this slot keeps its length
+    } else {
+      for (int e = 0; e < m; ++e) {
+        const int q = __ldcg(spare + rank + e);
+        s.table[long(i) * s.width + have + e] = q;
+        s.refs[q] = 1;
+      }
+      if (add[i]) s.lens[i] = len + add[i];
+    }
+    rank += max(0, m);
+  }
+}
+
+// ---- free ----------------------------------------------------------------------
+
+__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+    free_meta_kernel(const PageState s, const int* __restrict__ seqs, int n) {
+  copy_state(s, meta_gid());
+  cluster_sync();
+  for (int i = meta_warp(); i < n; i += kMetaWarps) {
+    const int slot = seqs[i], lane = threadIdx.x % 32;
+    if (slot < 0 || slot >= s.slots) {
+      if (lane == 0) report(s.err, kErrBounds);
+      continue;
+    }
+    // A slot that the list names twice is freed once.
+    const int had = __shfl_sync(0xffffffffu, lane == 0 ? atomicExch(s.lens + slot, 0) : 0, 0);
+    if (had <= 0) continue;
+    int* row = s.table + long(slot) * s.width;
+    for (int e = lane; e < s.width; e += 32) {
+      const int q = __ldcg(row + e);
+      if (q >= 0 && q < s.pages) atomicSub(s.refs + q, 1);
+      row[e] = -1;
+    }
+  }
+}
+
+// ---- compact -------------------------------------------------------------------
+
+// The L pages in use get the numbers below L: those that have one keep it, the
+// i-th of the others (ascending) moves to the i-th free page below L.
+// ws lists (pages each): pair sources, pair targets, sources from the last one
+// down, new number of each page.
+__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+    compact_meta_kernel(const PageState s, int* ws) {
+  __shared__ int sm[32];
+  const int gid = meta_gid();
+  int *src = ws + kListAt, *dst = src + s.pages, *down = dst + s.pages, *to = down + s.pages;
+  copy_state(s, gid);
+  int lo, hi, live;
+  int r = live_before(s.refs_in, s.pages, gid, sm, ws, lo, hi, live);
+  if (gid == 0 && live == s.pages) ws[kWsPairs] = 0;
+  for (int p = lo; p < hi; ++p) {
+    const bool used = s.refs_in[p] > 0;
+    to[p] = p;
+    if (p == live) ws[kWsPairs] = live - r;
+    if (!used && p < live) dst[p - r] = p;
+    if (used && p >= live) down[live - 1 - r] = p;
+    r += used;
+  }
+  cluster_sync();
+  const int pairs = __ldcg(ws + kWsPairs);
+  for (int i = gid; i < pairs; i += kMetaAll) {
+    const int from = __ldcg(down + pairs - 1 - i), t = __ldcg(dst + i);
+    src[i] = from;
+    to[from] = t;
+    s.refs[t] = s.refs_in[from];
+    s.refs[from] = 0;
+  }
+  cluster_sync();
+  for (long i = gid; i < long(s.slots) * s.width; i += kMetaAll) {
+    const int q = s.table_in[i];
+    if (q >= 0 && q < s.pages) s.table[i] = __ldcg(to + q);
+  }
+}
+
+// ---- copies of pages -------------------------------------------------------------
+
+struct CopyArgs {
+  char *k, *v;
+  long k_layer, k_page, v_layer, v_page;  // bytes
+  const int *src, *dst, *rows;            // rows null: whole pages
+  const int* count;                       // null: n pairs
+  int n, layers, heads, page, row_bytes, pages;
+  int* err;
+};
+
+constexpr int kCopyThreads = 256;
+
+// A warp copies the rows of one (pair, layer, k or v, head): up to 2 KB of
+// loads in flight, neighbouring warps on neighbouring heads of a page.
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs a) {
+  const int lane = threadIdx.x % 32;
+  const long warps = long(gridDim.x) * (kCopyThreads / 32);
+  const int n = a.count ? min(*a.count, a.n) : a.n;
+  const long units = long(n) * a.layers * 2 * a.heads;
+  for (long u = long(blockIdx.x) * (kCopyThreads / 32) + threadIdx.x / 32; u < units; u += warps) {
+    const int head = int(u % a.heads);
+    long w = u / a.heads;
+    const bool is_v = w & 1;
+    w >>= 1;
+    const int layer = int(w % a.layers), pair = int(w / a.layers);
+    const int from = a.src[pair], to = a.dst[pair];
+    if (from < 0) continue;
+    if (from >= a.pages || to < 0 || to >= a.pages) {
+      if (lane == 0) report(a.err, kErrBounds);
+      continue;
+    }
+    char* base = (is_v ? a.v + layer * a.v_layer : a.k + layer * a.k_layer) + long(head) * a.page * a.row_bytes;
+    const long stride = is_v ? a.v_page : a.k_page;
+    const uint4* in = reinterpret_cast<const uint4*>(base + from * stride);
+    uint4* out = reinterpret_cast<uint4*>(base + to * stride);
+    const int vecs = (a.rows ? a.rows[pair] : a.page) * (a.row_bytes / 16);
+    for (int i = lane; i < vecs; i += 128) {
+      uint4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + 32 * j < vecs) x[j] = in[i + 32 * j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + 32 * j < vecs) out[i + 32 * j] = x[j];
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+void check_int_vec(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous(), name,
+              ": must be contiguous int32 on ", place(like));
+}
+
+PageState state_of(const torch::Tensor& table, const torch::Tensor& lens, const torch::Tensor& refs,
+                   const torch::Tensor& table_out, const torch::Tensor& lens_out, const torch::Tensor& refs_out,
+                   int64_t page, const char* op) {
+  TORCH_CHECK(table.is_cuda(), op, ": table must be on a GPU");
+  TORCH_CHECK(table.dim() == 2 && lens.dim() == 1 && refs.dim() == 1 && lens.size(0) == table.size(0), op,
+              ": expected table (slots, width), lens (slots), refs (pages), got ", dims(table), ", ", dims(lens),
+              ", ", dims(refs));
+  for (const auto* t : {&table, &lens, &refs, &table_out, &lens_out, &refs_out}) check_int_vec(*t, op, table);
+  TORCH_CHECK(table_out.sizes() == table.sizes() && lens_out.sizes() == lens.sizes() &&
+                  refs_out.sizes() == refs.sizes(), op, ": shapes of the outputs");
+  const bool in_place = table_out.data_ptr() == table.data_ptr();
+  TORCH_CHECK(table.numel() == 0 || ((lens_out.data_ptr() == lens.data_ptr()) == in_place &&
+                                     (refs_out.data_ptr() == refs.data_ptr()) == (in_place || refs.numel() == 0)),
+              op, ": table, lens and refs are written all in place or all out of place");
+  TORCH_CHECK(page >= 1 && table.size(0) <= INT32_MAX / 8 && refs.size(0) <= INT32_MAX / 8 &&
+                  table.size(1) * page <= INT32_MAX, op, ": sizes");
+  return PageState{table.data_ptr<int>(), lens.data_ptr<int>(), refs.data_ptr<int>(), table_out.data_ptr<int>(),
+                   lens_out.data_ptr<int>(), refs_out.data_ptr<int>(), int(table.size(0)), int(table.size(1)),
+                   int(refs.size(0)), int(page), error_word()};
+}
+
+CopyArgs pools_of(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& like, const char* op) {
+  for (const auto* t : {&k, &v}) {
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), op, ": pages must be on ", place(like));
+    TORCH_CHECK(t->dim() == 5 && t->sizes() == k.sizes() && t->scalar_type() == k.scalar_type(), op,
+                ": pages must be (layers, pages, kv heads, rows, head_dim), k and v alike, got ", dims(*t));
+    TORCH_CHECK(t->stride(4) == 1 && t->stride(3) == t->size(4) && t->stride(2) == t->size(3) * t->size(4), op,
+                ": a page must be contiguous");
+    const int64_t es = t->element_size();
+    TORCH_CHECK(t->size(4) * es % 16 == 0 && t->stride(0) * es % 16 == 0 && t->stride(1) * es % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                op, ": rows of a page must be 16-byte aligned multiples of 16 bytes");
+  }
+  CopyArgs a{};
+  const int64_t es = k.element_size();
+  a.k = static_cast<char*>(k.data_ptr());
+  a.v = static_cast<char*>(v.data_ptr());
+  a.k_layer = k.stride(0) * es;
+  a.k_page = k.stride(1) * es;
+  a.v_layer = v.stride(0) * es;
+  a.v_page = v.stride(1) * es;
+  a.layers = int(k.size(0));
+  a.pages = int(k.size(1));
+  a.heads = int(k.size(2));
+  a.page = int(k.size(3));
+  a.row_bytes = int(k.size(4) * es);
+  a.err = error_word();
+  return a;
+}
+
+void launch_copy(const CopyArgs& a) {
+  const int64_t units = int64_t(a.n) * a.layers * 2 * a.heads;
+  if (units == 0) return;
+  const int64_t blocks = std::min<int64_t>((units + kCopyThreads / 32 - 1) / (kCopyThreads / 32), 148 * 8);
+  copy_pages_kernel<<<unsigned(blocks), kCopyThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "copy_pages launch failed");
+}
+
+torch::Tensor workspace(const torch::Tensor& like, int64_t ints) {
+  return torch::empty({kListAt + ints}, like.options());
+}
+
+}  // namespace
+
+void pages_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
+                torch::Tensor parents, torch::Tensor children, torch::Tensor table_out, torch::Tensor lens_out,
+                torch::Tensor refs_out) {
+  CopyArgs c = pools_of(k, v, table, "fork_pages");
+  const PageState s = state_of(table, lens, refs, table_out, lens_out, refs_out, c.page, "fork_pages");
+  TORCH_CHECK(c.pages == s.pages, "fork_pages: refs counts ", num(s.pages), " pages, the pool has ", num(c.pages));
+  check_int_vec(parents, "fork_pages: parents", table);
+  check_int_vec(children, "fork_pages: children", table);
+  TORCH_CHECK(parents.dim() == 1 && parents.sizes() == children.sizes(), "fork_pages: one parent for each child");
+  const int n = int(parents.size(0));
+  const at::cuda::CUDAGuard guard(table.device());
+  auto ws = workspace(table, s.slots + 5 * int64_t(n));
+  int* w = ws.data_ptr<int>();
+  fork_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
+      s, parents.data_ptr<int>(), children.data_ptr<int>(), n, w);
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fork_pages launch failed");
+  c.src = w + kListAt + s.slots + n;
+  c.dst = c.src + n;
+  c.rows = c.dst + n;
+  c.n = n;
+  launch_copy(c);
+}
+
+void pages_grow(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor add, int64_t page,
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out) {
+  const PageState s = state_of(table, lens, refs, table_out, lens_out, refs_out, page, "grow_pages");
+  check_int_vec(add, "grow_pages: add", table);
+  TORCH_CHECK(add.sizes() == lens.sizes(), "grow_pages: add must have one entry for each slot");
+  const at::cuda::CUDAGuard guard(table.device());
+  auto ws = workspace(table, s.pages);
+  grow_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(s, add.data_ptr<int>(),
+                                                                                     ws.data_ptr<int>());
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "grow_pages launch failed");
+}
+
+void pages_free(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor seqs,
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out) {
+  const PageState s = state_of(table, lens, refs, table_out, lens_out, refs_out, 1, "free_pages");
+  check_int_vec(seqs, "free_pages: seqs", table);
+  TORCH_CHECK(seqs.dim() == 1, "free_pages: seqs must be a vector");
+  const at::cuda::CUDAGuard guard(table.device());
+  free_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(s, seqs.data_ptr<int>(),
+                                                                                     int(seqs.size(0)));
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "free_pages launch failed");
+}
+
+void pages_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
+                   torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out) {
+  CopyArgs c = pools_of(k, v, table, "compact_pages");
+  const PageState s = state_of(table, lens, refs, table_out, lens_out, refs_out, c.page, "compact_pages");
+  TORCH_CHECK(c.pages == s.pages, "compact_pages: refs counts ", num(s.pages), " pages, the pool has ", num(c.pages));
+  const at::cuda::CUDAGuard guard(table.device());
+  auto ws = workspace(table, 4 * int64_t(s.pages));
+  int* w = ws.data_ptr<int>();
+  compact_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(s, w);
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "compact_pages launch failed");
+  c.src = w + kListAt;
+  c.dst = c.src + s.pages;
+  c.count = w + kWsPairs;
+  c.n = s.pages / 2;  // a move needs a page in use above and a free one below
+  launch_copy(c);
+}
+
+// Pages dst[i] = pages src[i] of every layer, k and v; pairs with a negative
+// source are skipped. No page may be both a source and a target.
+void pages_copy(torch::Tensor k, torch::Tensor v, torch::Tensor src, torch::Tensor dst) {
+  TORCH_CHECK(src.is_cuda(), "copy_pages: src must be on a GPU");
+  CopyArgs c = pools_of(k, v, src, "copy_pages");
+  check_int_vec(src, "copy_pages: src", src);
+  check_int_vec(dst, "copy_pages: dst", src);
+  TORCH_CHECK(src.dim() == 1 && src.sizes() == dst.sizes(), "copy_pages: one target for each source");
+  const at::cuda::CUDAGuard guard(src.device());
+  c.src = src.data_ptr<int>();
+  c.dst = dst.data_ptr<int>();
+  c.n = int(src.size(0));
+  launch_copy(c);
+}
+
+}  // namespace nk

@@ -1,0 +1,171 @@
+"""Paged KV cache operators (kernels: ``csrc/kernels/pages.cu``,
+``csrc/kernels/rotary.cu``, ``csrc/kernels/paged_attn.cu``).
+
+A cache is a pool of pages, ``k`` and ``v`` of shape (layers, pages, kv heads,
+rows of a page, head_dim), and three int32 tensors on the device:
+
+* ``table`` (slots, width)  the pages of each slot's sequence in order, -1 past the last
+* ``lens``  (slots)         its tokens; 0 means the slot is empty
+* ``refs``  (pages)         how many table entries name the page; 0 means it is free
+
+Sequences that were forked from one another share their full pages; a partly
+filled page belongs to one sequence, so appending never needs a copy. The state
+operators return ``(table, lens, refs)``; ``out`` takes three tensors for the
+result, which may be the inputs themselves (in place) and are fresh ones by
+default. No operator waits for the device: pages that run out or an index out
+of range are reported by ``kernel_status`` and the entry concerned is skipped.
+"""
+from typing import Optional, Sequence, Tuple, Union
+
+import numpy as np
+import torch
+
+from . import rotary
+from ._ext import ext
+
+State = Tuple[torch.Tensor, torch.Tensor, torch.Tensor]
+
+
+def _out(table, lens, refs, out) -> State:
+    return (torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)) if out is None else out
+
+
+def fork_pages(k, v, table, lens, refs, parents, children, out: Optional[State] = None) -> State:
+    """Make slot ``children[i]`` (empty; int32) a copy of slot ``parents[i]``.
+    Full pages are shared; the filled rows of a partly filled last page go to
+    the lowest free page, in the list's order. A child that is not empty, named
+    twice (its first mention counts), out of range or without a page to be had
+    is skipped and reported."""
+    out = _out(table, lens, refs, out)
+    ext().pages_fork(k, v, table, lens, refs, parents, children, *out)
+    return out
+
+
+def grow_pages(table, lens, refs, add, page: int, out: Optional[State] = None) -> State:
+    """Make room for ``add[s]`` (int32, one a slot) more tokens in every slot:
+    ``lens`` grows by it and missing pages are the lowest free ones, in the
+    order of the slots. A slot whose pages are not to be had keeps its length
+    and is reported."""
+    out = _out(table, lens, refs, out)
+    ext().pages_grow(table, lens, refs, add, page, *out)
+    return out
+
+
+def free_pages(table, lens, refs, seqs, out: Optional[State] = None) -> State:
+    """Empty the slots ``seqs`` (int32); pages that nobody else holds are free."""
+    out = _out(table, lens, refs, out)
+    ext().pages_free(table, lens, refs, seqs, *out)
+    return out
+
+
+def compact_pages(k, v, table, lens, refs, out: Optional[State] = None) -> State:
+    """Move pages so that the L ones in use are the first L of the pool: the
+    i-th page in use past L (ascending) takes the i-th free number below L."""
+    out = _out(table, lens, refs, out)
+    ext().pages_compact(k, v, table, lens, refs, *out)
+    return out
+
+
+def copy_pages(k, v, src, dst) -> None:
+    """Copy pages ``src[i]`` to ``dst[i]`` (int32) in every layer of k and v.
+    Pairs with a negative source are skipped; no page may be both a source and
+    a target, nor a target twice."""
+    ext().pages_copy(k, v, src, dst)
+
+
+SMALL_ROWS, ITEM_ROWS = 16, 64  # as in csrc/kernels/paged_attn.cu
+
+
+class PrefixPlan:
+    """Which rows belong to which sequence and which sequences share a prefix.
+
+    ``groups`` lists (sequences, shared tokens): so many sequences, one after
+    another, whose first ``shared`` tokens (whole pages) lie in the same pages.
+    ``q_lens`` is the number of new tokens of each sequence (one number for
+    all, or a list); the rows of q, k and v hold them one sequence after another.
+    ``slots`` names each sequence's row of the cache's table (0, 1, 2, ... by
+    default). A plan depends on nothing that changes from step to step, so one
+    plan serves every layer and every step of a batch, and a captured graph."""
+
+    def __init__(self, groups: Sequence[Tuple[int, int]], q_lens: Union[int, Sequence[int]] = 1, *, n_head: int,
+                 n_kv_head: int, head_dim: int, page: int, table_width: int, slots: Optional[Sequence[int]] = None,
+                 device="cuda"):
+        n_seq = sum(n for n, _ in groups)
+        if n_kv_head <= 0 or n_head % n_kv_head:
+            raise ValueError(f"{n_head} query heads cannot share {n_kv_head} kv heads")
+        if any(n < 0 or s < 0 or s % page or s > table_width * page for n, s in groups):
+            raise ValueError(f"groups must be (sequences, shared tokens), shared a multiple of the page ({page}) within "
+                             f"the table ({table_width} pages): {list(groups)}")
+        t = np.full(n_seq, q_lens, np.int64) if isinstance(q_lens, int) else np.asarray(list(q_lens), np.int64)
+        if len(t) != n_seq or (t < 0).any():
+            raise ValueError(f"q_lens must be one length for each of the {n_seq} sequences")
+        slot = np.arange(n_seq) if slots is None else np.asarray(list(slots), np.int64)
+        if len(slot) != n_seq or (slot < 0).any():
+            raise ValueError(f"slots must be one table row for each of the {n_seq} sequences")
+        share = n_head // n_kv_head
+        self.rows, self.share, self.max_slot = int(t.sum()), share, int(slot.max(initial=-1))
+        self.n_head, self.n_kv_head, self.head_dim, self.page, self.table_width = (n_head, n_kv_head, head_dim, page,
+                                                                                   table_width)
+        start = np.concatenate([[0], np.cumsum(t)])
+        seq = np.repeat(np.arange(n_seq), t)
+        back = start[seq + 1] - 1 - np.arange(self.rows)
+        items, of_pair = [], np.full((2, self.rows * share), -1, np.int64)
+
+        def add(shared, first, count, row0, row1, key0, keys):
+            pairs = (row1 - row0) * share
+            small = pairs <= SMALL_ROWS
+            for r in range(0, pairs, SMALL_ROWS if small else ITEM_ROWS):
+                n = min(ITEM_ROWS, pairs - r)
+                p0 = row0 * share + r
+                of_pair[shared, p0:p0 + n] = len(items)
+                after = keys if shared else back[(p0 + n - 1) // share]
+                items.append((shared, first, count, p0, n, key0, after, int(small)))
+
+        at = 0
+        own_from = np.zeros(n_seq, np.int64)
+        for n, shared in groups:
+            if n > 1 and shared > 0:  # one sequence has nothing to share
+                add(1, at, n, start[at], start[at + n], 0, shared)
+                own_from[at:at + n] = shared
+            at += n
+        for s in range(n_seq):
+            add(0, slot[s], 1, start[s], start[s + 1], own_from[s], 0)
+
+        def dev(x):
+            return torch.as_tensor(np.ascontiguousarray(x), dtype=torch.int32).to(device)
+
+        self.items = dev(np.asarray(items, np.int64).reshape(-1, 8))
+        self.shared_item, self.own_item = dev(of_pair[1]), dev(of_pair[0])
+        self.slot_of_seq, self.row_slot, self.row_back = dev(slot), dev(slot[seq]), dev(back)
+
+
+def append(q, k, v, k_pages, v_pages, table, lens, plan: PrefixPlan, cos=None, sin=None, layout: str = "half",
+           qk_eps: Optional[float] = None, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Write the new tokens' keys and values into one layer's pages (pages, kv
+    heads, rows of a page, head_dim), turned by their positions (``cos``,
+    ``sin`` of ``rotary.tables``; none: not turned) and, with ``qk_eps``, each
+    head of q and k divided by its root mean square as the model does after
+    RoPE (rs-nanogpt src/model/attention.rs:68-116). ``lens`` counts the new
+    tokens already (``grow_pages`` comes first). Returns q, turned and normed
+    alike, in ``q_out`` (which may be q)."""
+    if q_out is None:
+        q_out = torch.empty_like(q)
+    ext().paged_append(q, k, v, k_pages, v_pages, table, lens, plan.row_slot, plan.row_back, cos, sin,
+                       rotary.interleaved(layout), 0.0 if qk_eps is None else qk_eps, qk_eps is not None, q_out)
+    return q_out
+
+
+def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[torch.Tensor] = None,
+              lse: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of the new tokens ``q`` (rows, heads, head_dim) over one
+    layer's pages, the keys that a group shares read once for all its rows.
+    ``lens`` counts the new tokens; the last of them sees all of its sequence. A
+    row without keys (an empty slot) gives 0. ``lse`` (rows, heads) fp32 takes
+    the log of each row's softmax sum (-inf without keys). ``scale`` is
+    1 / sqrt(head_dim) by default."""
+    if out is None:
+        out = torch.empty_like(q)
+    ext().paged_attention(q, k_pages, v_pages, table, lens, plan.items, plan.slot_of_seq, plan.row_slot, plan.row_back,
+                          plan.shared_item, plan.own_item, plan.max_slot,
+                          q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
+    return out
