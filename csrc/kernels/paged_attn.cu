@@ -22,13 +22,13 @@
 // far below what the loads take for few rows.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <cuda_fp16.h>
 #include <torch/extension.h>
 
 #include <climits>
 
 #include "flash_common.cuh"
 #include "message.h"
+#include "paged_attn.cuh"
 #include "status.h"
 #include "tma_host.h"
 
@@ -44,63 +44,12 @@ constexpr int kMaxBoxes = 8;      // pages of a tile (page of 8 rows)
 constexpr int kSmallRows = 16;    // items up to here split the keys over the warps
 constexpr int kItemRows = 64;
 
-// One item, eight int32 (laid out by the host).
-struct Item {
-  int shared;  // 1: the shared pages of a group, 0: the rest of a sequence
-  int first;   // shared: first sequence of the group; else the slot
-  int count;   // shared: sequences of the group
-  int row0;    // first (row, query head) pair: row * share + head
-  int rows;    // pairs
-  int key0;    // first key
-  int keys;    // shared: number of keys; else the tokens that follow the item's last row
-  int small;   // keys are split over the warps
-};
-
 struct Tile {
   int item, head, key0, valid;  // valid: keys of the tile that are loaded
   int flags, row0, rows, small;
   int box[kMaxBoxes];           // page of each box
 };
 constexpr int kFirst = 1, kLast = 2, kContinued = 4;  // of the CTA's piece of the item
-
-struct Args {
-  const void* q;
-  long q_row, q_head;
-  const int *table, *lens;
-  int slots, width, page, pages;
-  const Item* items;
-  int n_items;
-  const int *slot_of_seq, *row_slot, *row_back;
-  int rows, share, hk;
-  float sl2;         // scale * log2(e)
-  float* part_o;     // (2, hk, rows * share, D), then (CTAs, 64, D)
-  float2* part_ml;   // the same without D: (max in base-2 units, sum)
-  int* tile0;        // n_items + 1: first tile of each item, of one head
-  int ctas;
-  int* err;
-};
-
-__device__ __forceinline__ int length_of(const Args& a, int slot) {
-  return min(max(a.lens[slot], 0), a.width * a.page);
-}
-
-__device__ __forceinline__ int tiles_of(const Args& a, const Item& it) {
-  const int keys = it.shared ? it.keys : length_of(a, it.first) - it.keys - it.key0;
-  return keys > 0 ? (keys + TK - 1) / TK : 0;
-}
-
-// CTA c's share of `total` tiles is [begin(c), begin(c + 1)); there are at most
-// as many shares as tiles.
-__device__ __forceinline__ int shares(int ctas, long total) { return int(total < ctas ? total : ctas); }
-__device__ __forceinline__ long share_begin(long c, int n, long total) { return c * total / n; }
-__device__ __forceinline__ int share_of(long t, int n, long total) { return int(((t + 1) * n - 1) / total); }
-
-__device__ __forceinline__ long base_slot(const Args& a, int shared, int head, int row) {
-  return (long(shared) * a.hk + head) * a.rows * a.share + row;
-}
-__device__ __forceinline__ long cta_slot(const Args& a, int cta, int r) {
-  return 2l * a.hk * a.rows * a.share + long(cta) * kItemRows + r;
-}
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1);
@@ -115,16 +64,6 @@ __device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&x)[4
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float x, float y) { return pack_bf16x2(x, y); }
-template <>
-__device__ __forceinline__ uint32_t pack<__half>(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 template <int D>
 struct Smem {
   static constexpr int kSub = TK * 128;             // 64 columns of a tile's rows, 128-byte swizzled
@@ -236,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_merge = reinterpret_cast<float*>(smem + kStages * 2 * S::kTile);
   __shared__ Tile ring[kRing];
-  __shared__ int s_sum[kThreads];
+  __shared__ int s_sum[kThreads + 1];
   __shared__ float s_ml[2][kSmallRows];
   __shared__ uint64_t full[kStages], empty[kStages], together;
 
@@ -249,42 +188,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(&together, kConsumers / 32);
     fence_barrier_init();
   }
-  // Tiles before each thread's run of items. CTA 0 leaves every item's first tile
-  // for the joining kernel.
-  const int per = (a.n_items + kThreads - 1) / kThreads;
-  const int i0 = min(a.n_items, tid * per), i1 = min(a.n_items, i0 + per);
-  int mine = 0;
-  for (int i = i0; i < i1; ++i) mine += tiles_of(a, a.items[i]);
-  s_sum[tid] = mine;
-  __syncthreads();
-  if (warp == 0) {
-    int run = 0;
-    for (int b = 0; b < kThreads; b += 32) {
-      const int v = s_sum[b + lane];
-      int x = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      s_sum[b + lane] = run + x - v;
-      run += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) s_ml[0][0] = __int_as_float(run);
-  }
-  __syncthreads();
-  const int head_tiles = __float_as_int(s_ml[0][0]);
-  __syncthreads();  // s_ml is free again
-  if (blockIdx.x == 0) {
-    int t = s_sum[tid];
-    for (int i = i0; i < i1; ++i) {
-      a.tile0[i] = t;
-      t += tiles_of(a, a.items[i]);
-    }
-    if (tid == 0) a.tile0[a.n_items] = head_tiles;
-  }
+  const Work& work = a.work[0];
+  const int head_tiles = deal<TK, kThreads>(a, work, s_sum);
   const long total = long(head_tiles) * a.hk;
-  const int n_shares = shares(a.ctas, total);
+  const int n_shares = shares(work.ctas, total);
   if (int(blockIdx.x) >= n_shares) return;
   const long t_begin = share_begin(blockIdx.x, n_shares, total);
   const int n_tiles = int(share_begin(blockIdx.x + 1, n_shares, total) - t_begin);
@@ -297,19 +204,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         Tile r;
         r.head = int(t / head_tiles);
         const int tt = int(t % head_tiles);
-        // The thread run that holds tile tt (the last whose first tile is not past it), then its item.
-        int lo = 0, hi = kThreads - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) / 2;
-          if (s_sum[mid] <= tt) lo = mid;
-          else hi = mid - 1;
-        }
-        int i = min(a.n_items, lo * per), at = s_sum[lo], n = tiles_of(a, a.items[i]);
-        while (at + n <= tt) {
-          at += n;
-          n = tiles_of(a, a.items[++i]);
-        }
-        const Item it = a.items[i];
+        int at, n;
+        const int i = item_of<TK, kThreads>(a, work, s_sum, tt, at, n);
+        const Item it = work.items[i];
         r.item = i;
         r.key0 = it.key0 + (tt - at) * TK;
         r.row0 = it.row0;
@@ -488,8 +385,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int e = 0; e < 2; ++e) {
       const int rr = wr + g + 8 * e;
       if (rr >= rows) continue;
-      const int shared = a.items[r.item].shared;
-      const long slot = continued ? cta_slot(a, blockIdx.x, rr) : base_slot(a, shared, head, row0 + rr);
+      const int shared = work.items[r.item].shared;
+      const long slot = continued ? cta_slot(work, blockIdx.x, rr) : base_slot(a, shared, head, row0 + rr);
       if (t4 == 0) a.part_ml[slot] = make_float2(acc.m[e], acc.l[e]);
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
@@ -499,65 +396,107 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// Joins the partials of every (row, query head): a warp each.
+// Joins the partials of every (row, query head): a warp each. A lane looks up one
+// partial, so their loads are in flight together, and the outputs are added with
+// the weights known.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const Args a, const int* __restrict__ shared_item,
                                                          const int* __restrict__ own_item, T* __restrict__ out,
                                                          long out_row, long out_head, float* __restrict__ lse) {
-  constexpr int E = D / 32;
-  pdl_wait();
-  const int w = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  constexpr int E = D / 32, U = 4;
+  const int wi = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   const int hq = a.hk * a.share;
-  if (w >= a.rows * hq) return;
-  const int row = w / hq, head = (w % hq) / a.share, pair = row * a.share + w % a.share;
-  const int head_tiles = a.tile0[a.n_items];
-  const long total = long(head_tiles) * a.hk;
-  const int n_shares = shares(a.ctas, total);
+  if (wi >= a.rows * hq) return;
+  const int row = wi / hq, head = (wi % hq) / a.share, pair = row * a.share + wi % a.share;
+  const int item[2] = {own_item[pair], shared_item[pair]};  // the plan's: no kernel before this one writes them
+  pdl_wait();
+  // Partials of either run: the first at its base slot, the others CTA by CTA.
+  int count[2] = {0, 0}, c0[2], r0[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (item[s] < 0) continue;
+    const Work& w = a.work[item[s] >= kBig];
+    const int i = item[s] % kBig, head_tiles = w.tile0[w.n];
+    const int first = w.tile0[i], n = w.tile0[i + 1] - first;
+    r0[s] = pair - w.items[i].row0;
+    if (n == 0) continue;
+    const long total = long(head_tiles) * a.hk, t = long(head) * head_tiles + first;
+    const int n_shares = shares(w.ctas, total);
+    c0[s] = share_of(t, n_shares, total);
+    count[s] = share_of(t + n - 1, n_shares, total) - c0[s] + 1;
+  }
   float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  auto join = [&](long slot) {
-    const float2 ml = a.part_ml[slot];
-    if (ml.x == -INFINITY && ml.y == 0.f) return;  // no key seen
-    const float mn = fmaxf(m, ml.x), x = exp2f(m - mn), y = exp2f(ml.x - mn);
-    m = mn;
-    l = l * x + ml.y * y;
-    const float* p = a.part_o + slot * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(p + e);
-      o[e] = o[e] * x + v.x * y;
-      o[e + 1] = o[e + 1] * x + v.y * y;
+  const int parts = count[0] + count[1];
+  for (int base = 0; base < parts; base += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    long slot = 0;
+    if (base + lane < parts) {
+      const int s = base + lane < count[0] ? 0 : 1, i = base + lane - (s ? count[0] : 0);
+      slot = i == 0 ? base_slot(a, s, head, pair) : cta_slot(a.work[item[s] >= kBig], c0[s] + i, r0[s]);
+      ml = a.part_ml[slot];
     }
-  };
+    float mx = ml.x;
 #pragma unroll
-  for (int s = 1; s >= 0; --s) {
-    const int i = s ? shared_item[pair] : own_item[pair];
-    if (i < 0) continue;
-    const int first = a.tile0[i], n = a.tile0[i + 1] - first;
-    if (n == 0) continue;
-    const long t = long(head) * head_tiles + first;
-    join(base_slot(a, s, head, pair));
-    const int c1 = share_of(t + n - 1, n_shares, total);
-    for (int c = share_of(t, n_shares, total) + 1; c <= c1; ++c) join(cta_slot(a, c, pair - a.items[i].row0));
+    for (int b = 16; b > 0; b >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+    mx = fmaxf(mx, m);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    // A partial that saw no key adds nothing, whatever its output holds.
+    const bool none = ml.x == -INFINITY && ml.y == 0.f;
+    const float weight = none ? 0.f : exp2f(ml.x - ref), before = exp2f(m - ref);
+    float sum = none ? 0.f : ml.y * weight;
+#pragma unroll
+    for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+    l = l * before + sum;
+    m = mx;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= before;
+    unsigned todo = __ballot_sync(0xffffffffu, !none);
+    while (todo) {
+      float x[U][E], wt[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int from = todo ? __ffs(todo) - 1 : 0;
+        wt[u] = __shfl_sync(0xffffffffu, weight, from);
+        const float* p = a.part_o + __shfl_sync(0xffffffffu, slot, from) * D + lane * E;
+        if (todo) {
+          if constexpr (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(p);
+            x[u][0] = v.x; x[u][1] = v.y;
+          }
+        } else {
+          wt[u] = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+        }
+        todo &= todo - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(x[u][e], wt[u], o[e]);
+    }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a NaN sum stays one
-  T* dst = out + row * out_row + (w % hq) * out_head + lane * E;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays one
+  T* dst = out + row * out_row + (wi % hq) * out_head + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + e) = pack<T>(l == 0.f ? 0.f : o[e] * inv, l == 0.f ? 0.f : o[e + 1] * inv);
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack<T>(o[e] * inv, o[e + 1] * inv);
   if (lse && lane == 0)
-    lse[long(row) * hq + w % hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    lse[long(row) * hq + wi % hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-CUtensorMap page_map(const torch::Tensor& t, const char* name) {
+CUtensorMap page_map(const torch::Tensor& t, int most_rows, const char* name) {
   const int64_t pages = t.size(0), heads = t.size(1), page = t.size(2), d = t.size(3);
   TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) * 2 % 16 == 0, name,
               ": pages must be 16-byte aligned");
   CUtensorMap m;
   const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads * page), cuuint64_t(pages)};
   const cuuint64_t strides[2] = {cuuint64_t(d * 2), cuuint64_t((pages > 1 ? t.stride(0) : heads * page * d) * 2)};
-  const cuuint32_t box[3] = {64, cuuint32_t(std::min<int64_t>(page, TK)), 1};
+  const cuuint32_t box[3] = {64, cuuint32_t(std::min<int64_t>(page, most_rows)), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const auto type = t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUresult r = encode_tiled_fn()(&m, type, 3, t.data_ptr(), dims, strides, box, estr,
@@ -568,7 +507,7 @@ CUtensorMap page_map(const torch::Tensor& t, const char* name) {
 }
 
 template <typename T, int D>
-void launch(const CUtensorMap& tk, const CUtensorMap& tv, Args& a, const int* shared_item, const int* own_item,
+void launch(const torch::Tensor& k, const torch::Tensor& v, Args& a, const int* shared_item, const int* own_item,
             torch::Tensor& out, float* lse) {
   constexpr int smem = Smem<D>::kBytes;
   static const bool configured = [] {
@@ -578,8 +517,14 @@ void launch(const CUtensorMap& tk, const CUtensorMap& tv, Args& a, const int* sh
   }();
   (void)configured;
   auto stream = at::cuda::getCurrentCUDAStream();
-  paged_attn_kernel<T, D><<<a.ctas, kThreads, smem, stream>>>(tk, tv, a);
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "paged_attention launch failed");
+  if (a.work[1].n)
+    launch_big<T, D>(page_map(k, kBigKeys, "paged_attention: k"), page_map(v, kBigKeys, "paged_attention: v"), a,
+                     stream);
+  if (a.work[0].n) {
+    paged_attn_kernel<T, D><<<a.work[0].ctas, kThreads, smem, stream>>>(page_map(k, TK, "paged_attention: k"),
+                                                                       page_map(v, TK, "paged_attention: v"), a);
+    TORCH_CHECK(cudaGetLastError() == cudaSuccess, "paged_attention launch failed");
+  }
   // The joining kernel is launched early and waits for the first one's results.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned((int64_t(a.rows) * a.hk * a.share + 7) / 8));
@@ -598,11 +543,12 @@ void launch(const CUtensorMap& tk, const CUtensorMap& tv, Args& a, const int* sh
 }  // namespace pa
 
 // q, out: (rows, query heads, head_dim); k, v: one layer's pages (pages, kv heads,
-// rows of a page, head_dim). items: (n, 8) int32, shared_item / own_item: item of
-// each (row, query head of a kv head), -1 where there is none.
+// rows of a page, head_dim). items, big_items: (n, 8) int32; shared_item, own_item:
+// item of each (row, query head of a kv head), plus kBig for big items, -1 where
+// there is none.
 void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
-                     torch::Tensor items, torch::Tensor slot_of_seq, torch::Tensor row_slot, torch::Tensor row_back,
-                     torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot, double scale,
+                     torch::Tensor items, torch::Tensor big_items, torch::Tensor slot_of_seq, torch::Tensor row_slot,
+                     torch::Tensor row_back,                    torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot, double scale,
                      torch::Tensor out, c10::optional<torch::Tensor> lse) {
   using namespace pa;
   const auto type = q.scalar_type();
@@ -628,7 +574,7 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   TORCH_CHECK(hk > 0 && hq % hk == 0, "paged_attention: ", num(hq), " query heads on ", num(hk), " kv heads");
   TORCH_CHECK(page >= 8 && (page & (page - 1)) == 0 && page <= 4096,
               "paged_attention: rows of a page must be a power of two from 8 to 4096, got ", num(page));
-  for (const auto* t : {&table, &lens, &items, &slot_of_seq, &row_slot, &row_back, &shared_item, &own_item})
+  for (const auto* t : {&table, &lens, &items, &big_items, &slot_of_seq, &row_slot, &row_back, &shared_item, &own_item})
     TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
                 "paged_attention: table, lens and the plan must be contiguous int32 on ", place(q));
   TORCH_CHECK(table.dim() == 2 && lens.dim() == 1 && table.size(0) == lens.size(0) && max_slot < table.size(0),
@@ -638,6 +584,7 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   const int64_t share = hq / hk;
   TORCH_CHECK(shared_item.numel() == rows * share, "paged_attention: the plan is for ",
               num(rows ? shared_item.numel() / rows : 0), " query heads a kv head, q has ", num(share));
+  TORCH_CHECK(scale > 0, "paged_attention: scale must be positive");
   TORCH_CHECK(rows * hq <= (int64_t(1) << 30) && table.size(1) * page <= INT32_MAX, "paged_attention: sizes");
   float* lse_p = nullptr;
   if (lse.has_value()) {
@@ -654,12 +601,9 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   a.q_head = q.stride(1);
   a.table = table.data_ptr<int>();
   a.lens = lens.data_ptr<int>();
-  a.slots = int(table.size(0));
   a.width = int(table.size(1));
   a.page = int(page);
   a.pages = int(k.size(0));
-  a.items = reinterpret_cast<const Item*>(items.data_ptr<int>());
-  a.n_items = int(items.size(0));
   a.slot_of_seq = slot_of_seq.data_ptr<int>();
   a.row_slot = row_slot.data_ptr<int>();
   a.row_back = row_back.data_ptr<int>();
@@ -667,21 +611,33 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   a.share = int(share);
   a.hk = int(hk);
   a.sl2 = float(scale * 1.4426950408889634);
-  a.ctas = 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.err = error_word();
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   // Partials and the items' first tiles, from the caching allocator: calls on
   // different streams do not share them.
-  const int64_t slots = 2 * rows * hq + int64_t(a.ctas) * kItemRows;
-  auto ws = torch::empty({slots * (d + 2) + a.n_items + 1}, q.options().dtype(at::kFloat));
+  int64_t slots = 2 * rows * hq, firsts = 0;
+  for (int i = 0; i < 2; ++i) {
+    const auto& list = i ? big_items : items;
+    Work& w = a.work[i];
+    w.items = reinterpret_cast<const Item*>(list.data_ptr<int>());
+    w.n = int(list.size(0));
+    w.ctas = i ? sms : 2 * sms;
+    w.item_rows = i ? kBigRows : kItemRows;
+    w.continued = slots;
+    if (w.n == 0) continue;
+    slots += int64_t(w.ctas) * w.item_rows;
+    firsts += w.n + 1;
+  }
+  auto ws = torch::empty({slots * (d + 2) + firsts}, q.options().dtype(at::kFloat));
   a.part_o = ws.data_ptr<float>();
   a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * d);
-  a.tile0 = reinterpret_cast<int*>(a.part_ml + slots);
-  const CUtensorMap tk = page_map(k, "paged_attention: k"), tv = page_map(v, "paged_attention: v");
+  a.work[0].tile0 = reinterpret_cast<int*>(a.part_ml + slots);
+  a.work[1].tile0 = a.work[0].tile0 + (a.work[0].n ? a.work[0].n + 1 : 0);
   const int *si = shared_item.data_ptr<int>(), *oi = own_item.data_ptr<int>();
-  if (type == at::kBFloat16 && d == 128) launch<__nv_bfloat16, 128>(tk, tv, a, si, oi, out, lse_p);
-  else if (type == at::kBFloat16) launch<__nv_bfloat16, 64>(tk, tv, a, si, oi, out, lse_p);
-  else if (d == 128) launch<__half, 128>(tk, tv, a, si, oi, out, lse_p);
-  else launch<__half, 64>(tk, tv, a, si, oi, out, lse_p);
+  if (type == at::kBFloat16 && d == 128) launch<__nv_bfloat16, 128>(k, v, a, si, oi, out, lse_p);
+  else if (type == at::kBFloat16) launch<__nv_bfloat16, 64>(k, v, a, si, oi, out, lse_p);
+  else if (d == 128) launch<__half, 128>(k, v, a, si, oi, out, lse_p);
+  else launch<__half, 64>(k, v, a, si, oi, out, lse_p);
 }
 
 }  // namespace nk

@@ -73,7 +73,10 @@ def copy_pages(k, v, src, dst) -> None:
     ext().pages_copy(k, v, src, dst)
 
 
-SMALL_ROWS, ITEM_ROWS = 16, 64  # as in csrc/kernels/paged_attn.cu
+# (row, query head) pairs of an item, as in csrc/kernels/paged_attn.cuh: up to
+# SMALL_ROWS on mma.sync with the keys split over the warps, up to ITEM_ROWS there
+# with the rows split, more on tcgen05, where 128 rows are one tile.
+SMALL_ROWS, ITEM_ROWS, BIG_ROWS, BIG = 16, 64, 256, 1 << 30
 
 
 class PrefixPlan:
@@ -94,8 +97,8 @@ class PrefixPlan:
         if n_kv_head <= 0 or n_head % n_kv_head:
             raise ValueError(f"{n_head} query heads cannot share {n_kv_head} kv heads")
         if any(n < 0 or s < 0 or s % page or s > table_width * page for n, s in groups):
-            raise ValueError(f"groups must be (sequences, shared tokens), shared a multiple of the page ({page}) within "
-                             f"the table ({table_width} pages): {list(groups)}")
+            raise ValueError(f"groups must be (sequences, shared tokens), shared a multiple of the page ({page}) "
+                             f"within the table ({table_width} pages): {list(groups)}")
         t = np.full(n_seq, q_lens, np.int64) if isinstance(q_lens, int) else np.asarray(list(q_lens), np.int64)
         if len(t) != n_seq or (t < 0).any():
             raise ValueError(f"q_lens must be one length for each of the {n_seq} sequences")
@@ -109,17 +112,18 @@ class PrefixPlan:
         start = np.concatenate([[0], np.cumsum(t)])
         seq = np.repeat(np.arange(n_seq), t)
         back = start[seq + 1] - 1 - np.arange(self.rows)
-        items, of_pair = [], np.full((2, self.rows * share), -1, np.int64)
+        lists, of_pair = ([], []), np.full((2, self.rows * share), -1, np.int64)
 
         def add(shared, first, count, row0, row1, key0, keys):
             pairs = (row1 - row0) * share
-            small = pairs <= SMALL_ROWS
-            for r in range(0, pairs, SMALL_ROWS if small else ITEM_ROWS):
-                n = min(ITEM_ROWS, pairs - r)
+            big = int(pairs > ITEM_ROWS)
+            items, most = lists[big], BIG_ROWS if big else ITEM_ROWS
+            for r in range(0, pairs, most):
+                n = min(most, pairs - r)
                 p0 = row0 * share + r
-                of_pair[shared, p0:p0 + n] = len(items)
+                of_pair[shared, p0:p0 + n] = len(items) + BIG * big
                 after = keys if shared else back[(p0 + n - 1) // share]
-                items.append((shared, first, count, p0, n, key0, after, int(small)))
+                items.append((shared, first, count, p0, n, key0, after, int(pairs <= SMALL_ROWS)))
 
         at = 0
         own_from = np.zeros(n_seq, np.int64)
@@ -134,7 +138,7 @@ class PrefixPlan:
         def dev(x):
             return torch.as_tensor(np.ascontiguousarray(x), dtype=torch.int32).to(device)
 
-        self.items = dev(np.asarray(items, np.int64).reshape(-1, 8))
+        self.items, self.big_items = (dev(np.asarray(x, np.int64).reshape(-1, 8)) for x in lists)
         self.shared_item, self.own_item = dev(of_pair[1]), dev(of_pair[0])
         self.slot_of_seq, self.row_slot, self.row_back = dev(slot), dev(slot[seq]), dev(back)
 
@@ -165,7 +169,7 @@ def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[
     1 / sqrt(head_dim) by default."""
     if out is None:
         out = torch.empty_like(q)
-    ext().paged_attention(q, k_pages, v_pages, table, lens, plan.items, plan.slot_of_seq, plan.row_slot, plan.row_back,
-                          plan.shared_item, plan.own_item, plan.max_slot,
+    ext().paged_attention(q, k_pages, v_pages, table, lens, plan.items, plan.big_items, plan.slot_of_seq, plan.row_slot,
+                          plan.row_back, plan.shared_item, plan.own_item, plan.max_slot,
                           q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
     return out

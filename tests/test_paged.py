@@ -343,7 +343,8 @@ CASES = {
     "plain paged": ([(1, 0)] * 5, [1, 63, 64, 65, 500], 1, 3, 3, 128, 64),
     "samples": ([(9, 192)], [1, 5, 64, 65, 30, 1, 200, 128, 63], 1, 4, 4, 128, 64),
     "one key past a tile": ([(3, 64)], [1, 1, 1], 1, 2, 1, 64, 16),
-    "ragged groups": ([(1, 32), (4, 96), (2, 0), (5, 16)], [7, 1, 33, 15, 16, 17, 90, 2, 3, 200, 1, 31], 1, 6, 3, 64, 16),
+    "ragged groups": ([(1, 32), (4, 96), (2, 0), (5, 16)], [7, 1, 33, 15, 16, 17, 90, 2, 3, 200, 1, 31], 1, 6, 3, 64,
+                      16),
     "many heads of one": ([(6, 128)], [9, 40, 3, 77, 1, 64], 1, 24, 2, 128, 32),
     "small pages": ([(3, 40)], [1, 9, 70], 1, 4, 2, 64, 8),
     "large pages": ([(20, 512)], list(range(1, 21)), 1, 2, 2, 128, 256),
@@ -353,6 +354,10 @@ CASES = {
     "a turn alone": ([(1, 0)], [300], [300], 2, 1, 128, 128),
     "long shares": ([(1, 0), (3, 20480)], [15000, 40, 7, 130], 1, 4, 2, 64, 64),
     "long shares of many rows": ([(2, 10240)], [70, 40], [33, 40], 10, 5, 64, 128),
+    "many rows of one prefix": ([(30, 256)], [1 + 11 * i % 140 for i in range(30)], 1, 8, 1, 128, 64),
+    "many rows, small heads and pages": ([(4, 40), (2, 1000)], [90, 200, 33, 129, 31, 64], [90, 150, 33, 128, 5, 64],
+                                         6, 2, 64, 8),
+    "a part of a tile": ([(1, 0), (1, 0)], [130, 257], [130, 129], 3, 1, 128, 256),
     "no new tokens for one": ([(3, 32)], [5, 20, 9], [1, 0, 2], 2, 2, 64, 32),
 }
 
@@ -570,7 +575,7 @@ def test_append_and_attention_refusals():
            lambda: call(q=q[..., :32]), lambda: call(k=k[:, :, :24], v=v[:, :, :24]), lambda: call(k=k[:, :1]),
            lambda: call(k=k.transpose(1, 2), v=v.transpose(1, 2)), lambda: call(t=t.long()), lambda: call(n=n[:1]),
            lambda: call(t=t[:1], n=n[:1]), lambda: call(plan=other), lambda: call(lse=torch.empty(2, 4)),
-           lambda: call(out=torch.empty_like(q).float()), lambda: call(q=q.cpu()),
+           lambda: call(out=torch.empty_like(q).float()), lambda: call(q=q.cpu()), lambda: call(scale=0.0),
            lambda: paged.append(q, kv[..., :32], kv, k, v, t, n, plan),
            lambda: paged.append(q, kv, kv[:, :1], k, v, t, n, plan),
            lambda: paged.append(q, kv, kv, k[..., :32], v, t, n, plan),
@@ -594,14 +599,14 @@ def test_plan_refusals_cpu(kw):
 def test_plan_items_cpu():
     """Every (row, head) pair is in one item of its own keys, and in one of the shared keys where its group shares."""
     from rs_nanogpt_b200.ops import paged
-    plan = paged.PrefixPlan([(1, 64), (3, 32), (2, 0)], [3, 40, 1, 0, 2, 5], n_head=6, n_kv_head=2, head_dim=64, page=32,
-                            table_width=8, device="cpu")
-    items = plan.items.tolist()
+    plan = paged.PrefixPlan([(1, 64), (3, 32), (2, 0)], [3, 40, 1, 0, 2, 5], n_head=6, n_kv_head=2, head_dim=64,
+                            page=32, table_width=8, device="cpu")
     seen = {0: [0] * (51 * 3), 1: [0] * (51 * 3)}
-    for i, (shared, first, count, row0, rows, key0, keys, small) in enumerate(items):
-        assert 0 < rows <= (16 if small else 64)
-        for p in range(row0, row0 + rows):
-            seen[shared][p] += 1
-            assert (plan.shared_item if shared else plan.own_item)[p] == i
+    for list_, most, mark in ((plan.items, 64, 0), (plan.big_items, 256, paged.BIG)):
+        for i, (shared, first, count, row0, rows, key0, keys, small) in enumerate(list_.tolist()):
+            assert 0 < rows <= (16 if small else most)
+            for p in range(row0, row0 + rows):
+                seen[shared][p] += 1
+                assert (plan.shared_item if shared else plan.own_item)[p] == i + mark
     assert seen[0] == [1] * 153
     assert seen[1] == [0] * 9 + [1] * (41 * 3) + [0] * 21
