@@ -15,11 +15,12 @@
 // a partial (max, sum, unnormalised output, fp32); a second kernel joins a row's
 // partials from the shared keys and from its own.
 //
-// CTA: a producer warp works out 32 tiles at a time (one a lane), then one thread
-// issues the TMA loads of a tile's pages; four warps compute on mma.sync, with the
-// running maximum and sum in registers. Items of up to 16 pairs (single tokens)
-// split a tile's keys over the warps, larger ones their rows. Tensor-core work is
-// far below what the loads take for few rows.
+// Here: items of up to 16 pairs (single tokens) on mma.sync, which is far from the
+// bound for so few rows; what counts is to keep loads in flight. A warp is a worker
+// of its own: it takes a share of the tiles, brings them into a two-stage ring of
+// its own by TMA and keeps the running maximum and sum in registers. No warp waits
+// for another, so the look-ups, first loads and write-outs of one run under the
+// loads of the others on its SM. Items of more pairs: paged_attn_tc.cu.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -27,6 +28,7 @@
 #include <climits>
 
 #include "flash_common.cuh"
+#include "launch.h"
 #include "message.h"
 #include "paged_attn.cuh"
 #include "status.h"
@@ -35,21 +37,9 @@
 namespace nk {
 namespace pa {
 
-constexpr int TK = 64;            // keys of a tile
-constexpr int kConsumers = 128;   // four warps
-constexpr int kThreads = kConsumers + 32;
-constexpr int kStages = 3;
-constexpr int kRing = 64;         // tile records, two batches of 32
-constexpr int kMaxBoxes = 8;      // pages of a tile (page of 8 rows)
-constexpr int kSmallRows = 16;    // items up to here split the keys over the warps
-constexpr int kItemRows = 64;
-
-struct Tile {
-  int item, head, key0, valid;  // valid: keys of the tile that are loaded
-  int flags, row0, rows, small;
-  int box[kMaxBoxes];           // page of each box
-};
-constexpr int kFirst = 1, kLast = 2, kContinued = 4;  // of the CTA's piece of the item
+constexpr int kWarps = 3;   // of a CTA; two CTAs an SM by shared memory
+constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 2;
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1);
@@ -64,22 +54,15 @@ __device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&x)[4
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
 }
+// A stage holds the K and V of TK keys, 16 KB: boxes of 32 or 64 rows by 128 bytes.
 template <int D>
-struct Smem {
-  static constexpr int kSub = TK * 128;             // 64 columns of a tile's rows, 128-byte swizzled
-  static constexpr int kTile = kSub * (D / 64);     // K or V of a tile
-  static constexpr int kMerge = kSmallRows * D * 4;
-  static constexpr int kBytes = 1024 + kStages * 2 * kTile + kMerge;
+struct Ring {
+  static constexpr int TK = 4096 / D;
+  static constexpr int kSub = TK * 128;          // 64 columns of the rows, 128-byte swizzled
+  static constexpr int kTile = kSub * (D / 64);  // K or V
+  static constexpr int kWarp = kStages * 2 * kTile;
+  static constexpr int kBytes = 1024 + kWarps * kWarp;
 };
-
-// Barrier of the four computing warps; like every wait it ends after a limit.
-__device__ __forceinline__ bool consumers_sync(uint64_t* bar, uint32_t& phase, int* err) {
-  __syncwarp();
-  if (threadIdx.x % 32 == 0) mbar_arrive(bar);
-  const bool ok = mbar_wait(bar, phase, kErrTimeoutOther, err);
-  phase ^= 1;
-  return ok;
-}
 
 // The state of a warp's 16 rows; thread (g, t4) holds rows g and g + 8.
 template <int D>
@@ -94,33 +77,33 @@ struct Acc {
   }
 };
 
-// Scores, softmax step and P V of one warp's 16 rows against NK keys of a tile,
-// from key k0 of it on. lim: keys of the tile that each of the two rows sees.
-template <typename T, int D, int NK>
-__device__ __forceinline__ void step(Acc<D>& acc, const uint32_t (&qf)[D / 16][4], uint32_t sK, uint32_t sV, int k0,
+// Scores, softmax step and P V of 16 rows against the TK keys of a stage. lim: keys
+// of the tile that each of the thread's two rows sees.
+template <typename T, int D>
+__device__ __forceinline__ void step(Acc<D>& acc, const uint32_t (&qf)[D / 16][4], uint32_t sK, uint32_t sV,
                                      const int (&lim)[2], float sl2) {
-  constexpr int kSub = Smem<D>::kSub;
+  constexpr int TK = Ring<D>::TK, kSub = Ring<D>::kSub;
   const int t4 = threadIdx.x & 3;
-  float s[NK / 8][4];
+  float s[TK / 8][4];
 #pragma unroll
-  for (int n = 0; n < NK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+  for (int n = 0; n < TK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-    for (int np = 0; np < NK / 16; ++np) {
+    for (int np = 0; np < TK / 16; ++np) {
       uint32_t b[4];
-      load_b_nk<64>(sK + (kk / 4) * kSub, k0 + np * 16, (kk % 4) * 16, b);
+      load_b_nk<64>(sK + (kk / 4) * kSub, np * 16, (kk % 4) * 16, b);
       mma<T>(s[2 * np], qf[kk], b[0], b[1]);
       mma<T>(s[2 * np + 1], qf[kk], b[2], b[3]);
     }
-  const bool masked = k0 + NK > min(lim[0], lim[1]);
+  const bool masked = TK > min(lim[0], lim[1]);
   float mx[2] = {acc.m[0], acc.m[1]};
 #pragma unroll
-  for (int n = 0; n < NK / 8; ++n)
+  for (int n = 0; n < TK / 8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       // A hidden score is replaced, whatever stood in its place.
-      const bool hide = masked && k0 + n * 8 + t4 * 2 + (e & 1) >= lim[e >> 1];
+      const bool hide = masked && n * 8 + t4 * 2 + (e & 1) >= lim[e >> 1];
       s[n][e] = hide ? -INFINITY : s[n][e] * sl2;
       mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
     }
@@ -143,168 +126,153 @@ __device__ __forceinline__ void step(Acc<D>& acc, const uint32_t (&qf)[D / 16][4
     acc.m[i] = mx[i];
   }
 #pragma unroll
-  for (int n = 0; n < NK / 8; ++n)
+  for (int n = 0; n < TK / 8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       s[n][e] = ex2_approx(s[n][e] - ref[e >> 1]);
       sum[e >> 1] += s[n][e];
     }
-  acc.l[0] += sum[0];  // this thread's columns; the quad's sums meet at the end of the item
+  acc.l[0] += sum[0];  // this thread's columns; the quad's sums meet at the end of the piece
   acc.l[1] += sum[1];
 #pragma unroll
-  for (int ks = 0; ks < NK / 16; ++ks) {
+  for (int ks = 0; ks < TK / 16; ++ks) {
     // P is rounded to the values' type for the tensor core; the sum keeps fp32.
     const uint32_t p[4] = {pack<T>(s[2 * ks][0], s[2 * ks][1]), pack<T>(s[2 * ks][2], s[2 * ks][3]),
                            pack<T>(s[2 * ks + 1][0], s[2 * ks + 1][1]), pack<T>(s[2 * ks + 1][2], s[2 * ks + 1][3])};
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) {
       uint32_t b[4];
-      load_b_kn<64>(sV + (n / 4) * kSub, (n % 4) * 16, k0 + ks * 16, b);
+      load_b_kn<64>(sV + (n / 4) * kSub, (n % 4) * 16, ks * 16, b);
       mma<T>(acc.o[2 * n], p, b[0], b[1]);
       mma<T>(acc.o[2 * n + 1], p, b[2], b[3]);
     }
   }
 }
 
+// A worker's place in its share: a piece is the part of an item that lies in it.
+struct Piece {
+  int left;  // tiles of the share that come after the piece
+  int head, index, tiles, key0, end, slot;  // end: keys of the item's run that exist
+  bool continued, whole;
+  Item item;
+};
+
+// The piece that begins at tile t, n_tiles before the share's end; by a whole warp.
+template <int TK>
+__device__ __forceinline__ Piece piece_at(const Args& a, const Work& w, const Deal<kThreads>& d, int head_tiles,
+                                          int t, int n_tiles) {
+  Piece p;
+  p.head = t / head_tiles;
+  const int tt = t % head_tiles;
+  int at, n;
+  p.index = item_of<TK, kThreads>(a, w, d, tt, at, n);
+  p.item = w.items[p.index];
+  p.tiles = min(n - (tt - at), n_tiles);
+  p.left = n_tiles - p.tiles;
+  p.key0 = p.item.key0 + (tt - at) * TK;
+  p.continued = tt != at;
+  p.whole = p.tiles == n;
+  run_end(a, p.item, p.slot, p.end);
+  return p;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const Args a) {
-  using S = Smem<D>;
+  using R = Ring<D>;
+  constexpr int TK = R::TK;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_merge = reinterpret_cast<float*>(smem + kStages * 2 * S::kTile);
-  __shared__ Tile ring[kRing];
-  __shared__ int s_sum[kThreads + 1];
-  __shared__ float s_ml[2][kSmallRows];
-  __shared__ uint64_t full[kStages], empty[kStages], together;
-
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kConsumers / 32);
-    }
-    mbar_init(&together, kConsumers / 32);
+  __shared__ Deal<kThreads> dealt;
+  __shared__ uint64_t s_full[kWarps][kStages];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)) +
+                  warp * R::kWarp;
+  uint64_t* full = s_full[warp];
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
   }
+  pdl_trigger();
   const Work& work = a.work[0];
-  const int head_tiles = deal<TK, kThreads>(a, work, s_sum);
-  const long total = long(head_tiles) * a.hk;
-  const int n_shares = shares(work.ctas, total);
-  if (int(blockIdx.x) >= n_shares) return;
-  const long t_begin = share_begin(blockIdx.x, n_shares, total);
-  const int n_tiles = int(share_begin(blockIdx.x + 1, n_shares, total) - t_begin);
-  const int box_rows = min(a.page, TK);
-
-  if (warp == kConsumers / 32) {
-    for (int base = 0; base < n_tiles; base += 32) {
-      if (base + lane < n_tiles) {
-        const long t = t_begin + base + lane;
-        Tile r;
-        r.head = int(t / head_tiles);
-        const int tt = int(t % head_tiles);
-        int at, n;
-        const int i = item_of<TK, kThreads>(a, work, s_sum, tt, at, n);
-        const Item it = work.items[i];
-        r.item = i;
-        r.key0 = it.key0 + (tt - at) * TK;
-        r.row0 = it.row0;
-        r.rows = it.rows;
-        r.small = it.small;
-        r.flags = (tt == at || base + lane == 0 ? kFirst : 0) |
-                  (tt == at + n - 1 || base + lane == n_tiles - 1 ? kLast : 0) |
-                  (tt != at && base + lane == 0 ? kContinued : 0);
-        int slot = it.first, end;
-        if (it.shared) {
-          // The shared pages are read through the first sequence that holds all of
-          // them, else through the longest (idle slots hold none).
-          int best = -1;
-          for (int s = it.first; s < it.first + it.count; ++s) {
-            const int c = a.slot_of_seq[s], len = length_of(a, c);
-            if (len > best) {
-              best = len;
-              slot = c;
-            }
-            if (len >= it.key0 + it.keys) break;
-          }
-          end = min(best, it.key0 + it.keys);
-        } else {
-          end = length_of(a, slot) - it.keys;
-        }
-        r.valid = min(TK, max(0, end - r.key0));
-#pragma unroll
-        for (int b = 0; b < kMaxBoxes; ++b) {
-          const int key = r.key0 + b * box_rows;
-          int page = 0;
-          if (b * box_rows < r.valid) {
-            page = a.table[long(slot) * a.width + key / a.page];
-            if (page < 0 || page >= a.pages) {
-              atomicCAS(a.err, 0, kErrBounds);
-              page = 0;
-            }
-          }
-          r.box[b] = page;
-        }
-        ring[(base + lane) % kRing] = r;
-      }
-      __syncwarp();
-      if (lane == 0) {
-        for (int i = base; i < min(n_tiles, base + 32); ++i) {
-          const int st = i % kStages;
-          if (!mbar_wait(&empty[st], ((i / kStages) & 1) ^ 1, kErrTimeoutProducer, a.err)) {
-            base = n_tiles;
-            break;
-          }
-          const Tile& r = ring[i % kRing];
-          const int boxes = (r.valid + box_rows - 1) / box_rows;
-          if (boxes == 0) {
-            mbar_arrive(&full[st]);
-            continue;
-          }
-          mbar_arrive_expect_tx(&full[st], boxes * box_rows * D * 2 * 2);
-          uint8_t* sK = smem + st * 2 * S::kTile;
-          for (int b = 0; b < boxes; ++b) {
-            const int row = r.head * a.page + (r.key0 + b * box_rows) % a.page;
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-              tma_load_3d(sK + c * S::kSub + b * box_rows * 128, &tm_k, &full[st], c * 64, row, r.box[b]);
-              tma_load_3d(sK + S::kTile + c * S::kSub + b * box_rows * 128, &tm_v, &full[st], c * 64, row, r.box[b]);
-            }
-          }
-        }
-      }
-      base = __shfl_sync(0xffffffffu, base, 0);
-    }
+  const int head_tiles = deal<TK, kThreads>(a, work, dealt);
+  const int total = head_tiles * a.hk, size = share_size(work.workers, total, work.least);
+  const int worker = warp * gridDim.x + blockIdx.x;  // few shares: spread over the SMs
+  const int t0 = worker * size, n_tiles = min(total - t0, size);
+  if (n_tiles <= 0) {
+    pdl_wait();
     return;
   }
+
+  // The loads run ahead of the computation by the ring's stages, with a cursor of
+  // their own (in, in_j); it holds the pages of up to 32 boxes of its piece, one a lane.
+  const int box_rows = min(a.page, TK), boxes_of_tile = TK / box_rows;
+  Piece in = piece_at<TK>(a, work, dealt, head_tiles, t0, n_tiles), now = in;
+  int in_j = 0, page = 0, page_from = 0;  // boxes [page_from, page_from + 32) of the piece are in `page`
+  auto look_up = [&](int box) {
+    page_from = box;
+    const int key = in.key0 + (box + lane) * box_rows;
+    page = 0;
+    if (key < in.end && box + lane < in.tiles * boxes_of_tile) {
+      page = a.table[long(in.slot) * a.width + key / a.page];
+      if (page < 0 || page >= a.pages) {
+        atomicCAS(a.err, 0, kErrBounds);
+        page = 0;
+      }
+    }
+  };
+  look_up(0);
+  int loaded = 0;
+  auto load_next = [&]() {
+    if (loaded == n_tiles) return;
+    if (in_j == in.tiles) {
+      in = piece_at<TK>(a, work, dealt, head_tiles, t0 + loaded, n_tiles - loaded);
+      in_j = 0;
+      look_up(0);
+    }
+    const int box0 = in_j * boxes_of_tile, k0 = in.key0 + in_j * TK;
+    if (box0 + boxes_of_tile > page_from + 32) look_up(box0);
+    const int boxes = k0 < in.end ? (min(in.end - k0, TK) + box_rows - 1) / box_rows : 0;
+    const int st = loaded % kStages;
+    if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * box_rows * D * 2 * 2);
+    __syncwarp();
+    // One lane a box: its page comes from the lane that looked it up.
+    const int pg = __shfl_sync(0xffffffffu, page, (box0 - page_from + lane) & 31);
+    if (lane < boxes) {
+      uint8_t* sK = ring + st * 2 * R::kTile + lane * box_rows * 128;
+      const int row = in.head * a.page + (k0 + lane * box_rows) % a.page;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_3d(sK + c * R::kSub, &tm_k, &full[st], c * 64, row, pg);
+        tma_load_3d(sK + R::kTile + c * R::kSub, &tm_v, &full[st], c * 64, row, pg);
+      }
+    }
+    ++in_j;
+    ++loaded;
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) load_next();
 
   const int g = lane >> 2, t4 = lane & 3;
   const T* Q = static_cast<const T*>(a.q);
   Acc<D> acc;
   uint32_t qf[D / 16][4];
   int lim[2];
-  uint32_t phase = 0;
-  bool continued = false;  // the piece at hand began in an earlier CTA
+  int j = now.tiles;  // so that the first tile begins a piece
   for (int i = 0; i < n_tiles; ++i) {
-    const int st = i % kStages;
-    if (!mbar_wait(&full[st], (i / kStages) & 1, kErrTimeoutMma, a.err)) break;
-    const Tile& r = ring[i % kRing];
-    const int flags = r.flags, rows = r.rows, row0 = r.row0, head = r.head, valid = r.valid, key0 = r.key0;
-    const bool small = r.small;
-    const int wr = small ? 0 : warp * 16;  // first row of this warp
-    if (flags & kFirst) {
+    if (j == now.tiles) {
+      if (i > 0) now = piece_at<TK>(a, work, dealt, head_tiles, t0 + i, n_tiles - i);
+      j = 0;
       acc.clear();
-      continued = flags & kContinued;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int rr = wr + g + 8 * e;
+        const int rr = g + 8 * e;
         lim[e] = INT_MAX / 2;  // rows past the item's: computed on zeros, never written
         const T* src = nullptr;
-        if (rr < rows) {
-          const int row = (row0 + rr) / a.share, h = (row0 + rr) % a.share;
+        if (rr < now.item.rows) {
+          const int row = (now.item.row0 + rr) / a.share, h = (now.item.row0 + rr) % a.share;
           lim[e] = length_of(a, a.row_slot[row]) - a.row_back[row];
-          src = Q + row * a.q_row + (head * a.share + h) * a.q_head;
+          src = Q + row * a.q_row + (now.head * a.share + h) * a.q_head;
         }
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -313,80 +281,44 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
-    const uint32_t sK = smem_u32(smem + st * 2 * S::kTile), sV = sK + S::kTile;
+    const int st = i % kStages, k0 = now.key0 + j * TK, valid = min(TK, max(0, now.end - k0));
+    if (!wait(&full[st], (i / kStages) & 1, kErrTimeoutMma, a.err)) return;
+    uint8_t* tile = ring + st * 2 * R::kTile;
     if (valid < TK) {
       // Rows past the last key hold what the page or an earlier tile held, which
       // may be anything: values are cleared, so that 0 * v is 0.
-      for (int c = tid; c < (TK - valid) * (D / 8); c += kConsumers) {
+      for (int c = lane; c < (TK - valid) * (D / 8); c += 32) {
         const int row = valid + c / (D / 8), ch = c % (D / 8);
-        uint8_t* at = smem + (st * 2 + 1) * S::kTile + (ch / 8) * S::kSub + row * 128 + (ch % 8) * 16;
-        *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(tile + R::kTile + (ch / 8) * R::kSub + row * 128 + (ch % 8) * 16) =
+            make_uint4(0, 0, 0, 0);
       }
-      if (!consumers_sync(&together, phase, a.err)) return;
+      __syncwarp();
     }
-    const int tl[2] = {min(lim[0] - key0, valid), min(lim[1] - key0, valid)};
-    if (small) {
-      step<T, D, 16>(acc, qf, sK, sV, warp * 16, tl, a.sl2);
-    } else if (wr < rows) {
-      step<T, D, TK>(acc, qf, sK, sV, 0, tl, a.sl2);
-    }
+    const int see[2] = {min(lim[0] - k0, valid), min(lim[1] - k0, valid)};
+    step<T, D>(acc, qf, smem_u32(tile), smem_u32(tile + R::kTile), see, a.sl2);
     if (valid < TK) fence_proxy_async();  // the clearing stores come before the next load into this stage
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[st]);
-    if (!(flags & kLast)) continue;
+    load_next();
+    if (++j < now.tiles) continue;
 
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       acc.l[e] += __shfl_xor_sync(0xffffffffu, acc.l[e], 1);
       acc.l[e] += __shfl_xor_sync(0xffffffffu, acc.l[e], 2);
-    }
-    if (small) {
-      // Warps 3, 2, 1 hand their rows down; warp 0 ends with all of them.
-#pragma unroll 1
-      for (int w = kConsumers / 32 - 1; w > 0; --w) {
-        if (warp == w) {
+      const int rr = g + 8 * e;
+      if (rr >= now.item.rows) continue;
+      if (now.item.alone && now.whole) {  // nothing to join
+        const int row = (now.item.row0 + rr) / a.share, h = now.head * a.share + (now.item.row0 + rr) % a.share;
+        const float inv = inverse(acc.l[e]);
+        T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + t4 * 2;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int rr = g + 8 * e;
-            if (rr >= rows) continue;
-            if (t4 == 0) {
-              s_ml[0][rr] = acc.m[e];
-              s_ml[1][rr] = acc.l[e];
-            }
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-              *reinterpret_cast<float2*>(s_merge + rr * D + n * 8 + t4 * 2) =
-                  make_float2(acc.o[n][2 * e], acc.o[n][2 * e + 1]);
-          }
-        }
-        if (!consumers_sync(&together, phase, a.err)) return;
-        if (warp == w - 1) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int rr = g + 8 * e;
-            if (rr >= rows) continue;
-            const float m2 = s_ml[0][rr], m = fmaxf(acc.m[e], m2), ref = m == -INFINITY ? 0.f : m;
-            const float x = exp2f(acc.m[e] - ref), y = exp2f(m2 - ref);
-            acc.m[e] = m;
-            acc.l[e] = acc.l[e] * x + s_ml[1][rr] * y;
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              const float2 o = *reinterpret_cast<const float2*>(s_merge + rr * D + n * 8 + t4 * 2);
-              acc.o[n][2 * e] = acc.o[n][2 * e] * x + o.x * y;
-              acc.o[n][2 * e + 1] = acc.o[n][2 * e + 1] * x + o.y * y;
-            }
-          }
-        }
-        if (!consumers_sync(&together, phase, a.err)) return;
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<uint32_t*>(dst + n * 8) = pack<T>(acc.o[n][2 * e] * inv, acc.o[n][2 * e + 1] * inv);
+        if (a.lse && t4 == 0) a.lse[long(row) * a.hk * a.share + h] = lse_of(acc.m[e], acc.l[e]);
+        continue;
       }
-    }
-    if (small && warp > 0) continue;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int rr = wr + g + 8 * e;
-      if (rr >= rows) continue;
-      const int shared = work.items[r.item].shared;
-      const long slot = continued ? cta_slot(work, blockIdx.x, rr) : base_slot(a, shared, head, row0 + rr);
+      const long slot = now.continued ? continued_slot(work, worker, now.item.row0 + rr)
+                                      : base_slot(a, now.item.shared, now.head, now.item.row0 + rr);
       if (t4 == 0) a.part_ml[slot] = make_float2(acc.m[e], acc.l[e]);
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
@@ -394,52 +326,55 @@ __global__ void __launch_bounds__(kThreads, 2)
             make_float2(acc.o[n][2 * e], acc.o[n][2 * e + 1]);
     }
   }
+  pdl_wait();  // started beside the kernel of the big items: it ends, and the join begins, after that one
 }
 
-// Joins the partials of every (row, query head): a warp each. A lane looks up one
-// partial, so their loads are in flight together, and the outputs are added with
-// the weights known.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const Args a, const int* __restrict__ shared_item,
-                                                         const int* __restrict__ own_item, T* __restrict__ out,
-                                                         long out_row, long out_head, float* __restrict__ lse) {
-  constexpr int E = D / 32, U = 4;
-  const int wi = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+// Joins the partials of every (row, query head) that the kernels above left in
+// several pieces: L lanes each. A lane looks up one partial, so their loads are in
+// flight together, and the outputs are added with the weights known. All 32 lanes
+// where there are few pairs and so many partials of each (latency counts), eight
+// where there are many pairs of few partials (loads in flight count).
+constexpr int kJoinThreads = 128;
+template <typename T, int D, int L>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, const int* __restrict__ shared_item,
+                                                                  const int* __restrict__ own_item) {
+  constexpr int E = D / L, U = 4 * L / 32 + 1, W = E < 4 ? E : 4;  // W: floats of a load
+  const int id = (blockIdx.x * kJoinThreads + threadIdx.x) / L, lane = threadIdx.x % L;
+  const unsigned lanes = (L == 32 ? 0xffffffffu : (1u << (L % 32)) - 1) << (threadIdx.x % 32 / L * L);
   const int hq = a.hk * a.share;
-  if (wi >= a.rows * hq) return;
-  const int row = wi / hq, head = (wi % hq) / a.share, pair = row * a.share + wi % a.share;
+  if (id >= a.rows * hq) return;  // by whole groups of lanes
+  const int row = id / hq, h = id % hq, head = h / a.share, pair = row * a.share + h % a.share;
   const int item[2] = {own_item[pair], shared_item[pair]};  // the plan's: no kernel before this one writes them
   pdl_wait();
-  // Partials of either run: the first at its base slot, the others CTA by CTA.
-  int count[2] = {0, 0}, c0[2], r0[2];
+  // Partials of either run: the first at its base slot, the others worker by worker.
+  int count[2] = {0, 0}, c0[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     if (item[s] < 0) continue;
-    const Work& w = a.work[item[s] >= kBig];
-    const int i = item[s] % kBig, head_tiles = w.tile0[w.n];
-    const int first = w.tile0[i], n = w.tile0[i + 1] - first;
-    r0[s] = pair - w.items[i].row0;
+    const Work& w = item[s] >= kBig ? a.work[1] : a.work[0];
+    const int i = item[s] & (kBig - 1), all = w.tile0[w.n], first = w.tile0[i], n = w.tile0[i + 1] - first;
     if (n == 0) continue;
-    const long total = long(head_tiles) * a.hk, t = long(head) * head_tiles + first;
-    const int n_shares = shares(w.ctas, total);
-    c0[s] = share_of(t, n_shares, total);
-    count[s] = share_of(t + n - 1, n_shares, total) - c0[s] + 1;
+    const int size = share_size(w.workers, all * a.hk, w.least), t = head * all + first;
+    c0[s] = t / size;
+    count[s] = (t + n - 1) / size - c0[s] + 1;
   }
+  const int parts = count[0] + count[1];
+  if (parts == 1 && (item[0] < 0 || item[1] < 0)) return;  // its only piece wrote the output
   float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  const int parts = count[0] + count[1];
-  for (int base = 0; base < parts; base += 32) {
+  for (int base = 0; base < parts; base += L) {
     float2 ml = make_float2(-INFINITY, 0.f);
     long slot = 0;
     if (base + lane < parts) {
       const int s = base + lane < count[0] ? 0 : 1, i = base + lane - (s ? count[0] : 0);
-      slot = i == 0 ? base_slot(a, s, head, pair) : cta_slot(a.work[item[s] >= kBig], c0[s] + i, r0[s]);
+      slot = i == 0 ? base_slot(a, s, head, pair)
+                    : continued_slot(item[s] >= kBig ? a.work[1] : a.work[0], c0[s] + i, pair);
       ml = a.part_ml[slot];
     }
     float mx = ml.x;
 #pragma unroll
-    for (int b = 16; b > 0; b >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+    for (int b = L / 2; b > 0; b >>= 1) mx = fmaxf(mx, __shfl_xor_sync(lanes, mx, b));
     mx = fmaxf(mx, m);
     const float ref = mx == -INFINITY ? 0.f : mx;
     // A partial that saw no key adds nothing, whatever its output holds.
@@ -447,33 +382,39 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Args a, const int
     const float weight = none ? 0.f : exp2f(ml.x - ref), before = exp2f(m - ref);
     float sum = none ? 0.f : ml.y * weight;
 #pragma unroll
-    for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+    for (int b = L / 2; b > 0; b >>= 1) sum += __shfl_xor_sync(lanes, sum, b);
     l = l * before + sum;
     m = mx;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= before;
-    unsigned todo = __ballot_sync(0xffffffffu, !none);
-    while (todo) {
+    const int n = min(L, parts - base);
+    for (int i = 0; i < n; i += U) {
       float x[U][E], wt[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int from = todo ? __ffs(todo) - 1 : 0;
-        wt[u] = __shfl_sync(0xffffffffu, weight, from);
-        const float* p = a.part_o + __shfl_sync(0xffffffffu, slot, from) * D + lane * E;
-        if (todo) {
-          if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p);
-            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(p);
-            x[u][0] = v.x; x[u][1] = v.y;
+        const int from = min(i + u, n - 1);
+        wt[u] = __shfl_sync(lanes, i + u < n ? weight : 0.f, from, L);
+        if (i + u >= n) wt[u] = 0.f;
+        const float* p = a.part_o + __shfl_sync(lanes, slot, from, L) * D + lane * W;
+        if (wt[u] != 0.f) {
+#pragma unroll
+          for (int e = 0; e < E; e += W) {
+            if constexpr (W == 4) {
+              const float4 v = *reinterpret_cast<const float4*>(p + e * L);
+              x[u][e] = v.x;
+              x[u][e + 1] = v.y;
+              x[u][e + 2] = v.z;
+              x[u][e + 3] = v.w;
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(p + e * L);
+              x[u][e] = v.x;
+              x[u][e + 1] = v.y;
+            }
           }
         } else {
-          wt[u] = 0.f;
 #pragma unroll
           for (int e = 0; e < E; ++e) x[u][e] = 0.f;
         }
-        todo &= todo - 1;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -481,12 +422,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const Args a, const int
         for (int e = 0; e < E; ++e) o[e] = fmaf(x[u][e], wt[u], o[e]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays one
-  T* dst = out + row * out_row + (wi % hq) * out_head + lane * E;
+  const float inv = inverse(l);
+  T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + lane * W;
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack<T>(o[e] * inv, o[e + 1] * inv);
-  if (lse && lane == 0)
-    lse[long(row) * hq + wi % hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + (e / W) * W * L + e % W) = pack<T>(o[e] * inv, o[e + 1] * inv);
+  if (a.lse && lane == 0) a.lse[long(row) * hq + h] = lse_of(m, l);
 }
 
 CUtensorMap page_map(const torch::Tensor& t, int most_rows, const char* name) {
@@ -507,9 +448,9 @@ CUtensorMap page_map(const torch::Tensor& t, int most_rows, const char* name) {
 }
 
 template <typename T, int D>
-void launch(const torch::Tensor& k, const torch::Tensor& v, Args& a, const int* shared_item, const int* own_item,
-            torch::Tensor& out, float* lse) {
-  constexpr int smem = Smem<D>::kBytes;
+void launch(const torch::Tensor& k, const torch::Tensor& v, const Args& a, const int* shared_item,
+            const int* own_item) {
+  constexpr int smem = Ring<D>::kBytes, TK = Ring<D>::TK;
   static const bool configured = [] {
     TORCH_CHECK(cudaFuncSetAttribute(paged_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
                     cudaSuccess, "paged_attention: shared memory");
@@ -517,27 +458,27 @@ void launch(const torch::Tensor& k, const torch::Tensor& v, Args& a, const int* 
   }();
   (void)configured;
   auto stream = at::cuda::getCurrentCUDAStream();
-  if (a.work[1].n)
+  const bool big = a.work[1].n, small = a.work[0].n;
+  if (big)
     launch_big<T, D>(page_map(k, kBigKeys, "paged_attention: k"), page_map(v, kBigKeys, "paged_attention: v"), a,
                      stream);
-  if (a.work[0].n) {
-    paged_attn_kernel<T, D><<<a.work[0].ctas, kThreads, smem, stream>>>(page_map(k, TK, "paged_attention: k"),
-                                                                       page_map(v, TK, "paged_attention: v"), a);
-    TORCH_CHECK(cudaGetLastError() == cudaSuccess, "paged_attention launch failed");
+  if (small) {
+    const dim3 grid(unsigned(a.work[0].workers / kWarps));
+    const CUtensorMap tk = page_map(k, TK, "paged_attention: k"), tv = page_map(v, TK, "paged_attention: v");
+    if (big) {  // reads nothing of the big items' kernel, so it may fill the SMs that one leaves free
+      TORCH_CHECK(launch_early(paged_attn_kernel<T, D>, grid, dim3(kThreads), smem, stream, tk, tv, a) == cudaSuccess,
+                  "paged_attention launch failed");
+    } else {
+      paged_attn_kernel<T, D><<<grid, kThreads, smem, stream>>>(tk, tv, a);
+      TORCH_CHECK(cudaGetLastError() == cudaSuccess, "paged_attention launch failed");
+    }
   }
-  // The joining kernel is launched early and waits for the first one's results.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned((int64_t(a.rows) * a.hk * a.share + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  TORCH_CHECK(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a, shared_item, own_item,
-                                 reinterpret_cast<T*>(out.data_ptr()), long(out.stride(0)), long(out.stride(1)), lse) ==
-                  cudaSuccess, "paged_attention: join launch failed");
+  const int64_t pairs = int64_t(a.rows) * a.hk * a.share;
+  const bool few = pairs <= 148 * 64;
+  const int64_t per = kJoinThreads / (few ? 32 : 8);
+  const auto join = few ? paged_join_kernel<T, D, 32> : paged_join_kernel<T, D, 8>;
+  TORCH_CHECK(launch_early(join, dim3(unsigned((pairs + per - 1) / per)), dim3(kJoinThreads), 0, stream, a, shared_item,
+                           own_item) == cudaSuccess, "paged_attention: join launch failed");
 }
 
 }  // namespace pa
@@ -548,8 +489,8 @@ void launch(const torch::Tensor& k, const torch::Tensor& v, Args& a, const int* 
 // there is none.
 void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                      torch::Tensor items, torch::Tensor big_items, torch::Tensor slot_of_seq, torch::Tensor row_slot,
-                     torch::Tensor row_back,                    torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot, double scale,
-                     torch::Tensor out, c10::optional<torch::Tensor> lse) {
+                     torch::Tensor row_back, torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot,
+                     double scale, torch::Tensor out, c10::optional<torch::Tensor> lse) {
   using namespace pa;
   const auto type = q.scalar_type();
   TORCH_CHECK(q.is_cuda(), "paged_attention: q must be on a GPU");
@@ -586,12 +527,10 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
               num(rows ? shared_item.numel() / rows : 0), " query heads a kv head, q has ", num(share));
   TORCH_CHECK(scale > 0, "paged_attention: scale must be positive");
   TORCH_CHECK(rows * hq <= (int64_t(1) << 30) && table.size(1) * page <= INT32_MAX, "paged_attention: sizes");
-  float* lse_p = nullptr;
   if (lse.has_value()) {
     TORCH_CHECK(lse->device() == q.device() && lse->scalar_type() == at::kFloat && lse->is_contiguous() &&
                     lse->dim() == 2 && lse->size(0) == rows && lse->size(1) == hq,
                 "paged_attention: lse must be contiguous fp32 (rows, heads)");
-    lse_p = lse->data_ptr<float>();
   }
   if (rows == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
@@ -611,6 +550,10 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   a.share = int(share);
   a.hk = int(hk);
   a.sl2 = float(scale * 1.4426950408889634);
+  a.out = out.data_ptr();
+  a.out_row = out.stride(0);
+  a.out_head = out.stride(1);
+  a.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
   a.err = error_word();
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   // Partials and the items' first tiles, from the caching allocator: calls on
@@ -621,11 +564,12 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
     Work& w = a.work[i];
     w.items = reinterpret_cast<const Item*>(list.data_ptr<int>());
     w.n = int(list.size(0));
-    w.ctas = i ? sms : 2 * sms;
-    w.item_rows = i ? kBigRows : kItemRows;
+    w.workers = i ? sms : 2 * kWarps * sms;
+    w.item_rows = i ? kBigRows : kSmallRows;
     w.continued = slots;
+    w.least = i ? 1 : 2;  // a share of one tile leaves more to join than it saves
     if (w.n == 0) continue;
-    slots += int64_t(w.ctas) * w.item_rows;
+    slots += int64_t(w.workers) * w.item_rows;
     firsts += w.n + 1;
   }
   auto ws = torch::empty({slots * (d + 2) + firsts}, q.options().dtype(at::kFloat));
@@ -634,10 +578,10 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   a.work[0].tile0 = reinterpret_cast<int*>(a.part_ml + slots);
   a.work[1].tile0 = a.work[0].tile0 + (a.work[0].n ? a.work[0].n + 1 : 0);
   const int *si = shared_item.data_ptr<int>(), *oi = own_item.data_ptr<int>();
-  if (type == at::kBFloat16 && d == 128) launch<__nv_bfloat16, 128>(k, v, a, si, oi, out, lse_p);
-  else if (type == at::kBFloat16) launch<__nv_bfloat16, 64>(k, v, a, si, oi, out, lse_p);
-  else if (d == 128) launch<__half, 128>(k, v, a, si, oi, out, lse_p);
-  else launch<__half, 64>(k, v, a, si, oi, out, lse_p);
+  if (type == at::kBFloat16 && d == 128) launch<__nv_bfloat16, 128>(k, v, a, si, oi);
+  else if (type == at::kBFloat16) launch<__nv_bfloat16, 64>(k, v, a, si, oi);
+  else if (d == 128) launch<__half, 128>(k, v, a, si, oi);
+  else launch<__half, 64>(k, v, a, si, oi);
 }
 
 }  // namespace nk

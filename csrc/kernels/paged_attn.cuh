@@ -21,19 +21,22 @@ struct Item {
   int rows;    // pairs
   int key0;    // first key
   int keys;    // shared: number of keys; else the tokens that follow the item's last row
-  int small;   // keys are split over the warps
+  int alone;   // its pairs have no other run of keys
 };
 
 // The items of one kernel. Their tiles are numbered one after another, head by
-// head, and every CTA takes an equal contiguous share of the numbers.
+// head, and every worker (a warp, or a CTA) takes an equal contiguous share of the
+// numbers.
 struct Work {
   const Item* items;
   int n;           // items of one head
-  int ctas;
+  int workers;
   int* tile0;      // n + 1: first tile of each item, of one head (written by CTA 0)
-  long continued;  // partial slots of the CTAs' pieces that continue an earlier CTA's
+  long continued;  // partial slots of the workers' pieces that continue an earlier worker's
   int item_rows;   // slots of each
+  int least;       // tiles of a share
 };
+constexpr int kSmallRows = 16;
 constexpr int kBig = 1 << 30;  // marks an item of work[1] in the join's lists
 
 struct Args {
@@ -47,8 +50,26 @@ struct Args {
   float* part_o;     // a partial output (D, unnormalised) a slot: (2, hk, rows * share), then the continued ones
   float2* part_ml;   // its maximum in base-2 units, and its sum
   Work work[2];      // on mma.sync, on tcgen05
+  void* out;
+  long out_row, out_head;
+  float* lse;        // may be null
   int* err;
 };
+
+// mbar_wait that polls for a while before it first reads the timer, which would
+// otherwise stand in the path of every wait that has to wait at all.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int code, int* err) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, code, err);
+}
+
+// 1 / sum; 0 for a row without keys, NaN where the sum is.
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
 
 __device__ __forceinline__ int length_of(const Args& a, int slot) {
   return min(max(a.lens[slot], 0), a.width * a.page);
@@ -60,75 +81,124 @@ __device__ __forceinline__ int tiles_of(const Args& a, const Item& it) {
   return keys > 0 ? (keys + TK - 1) / TK : 0;
 }
 
-// CTA c's share of `total` tiles is [begin(c), begin(c + 1)); there are at most
-// as many shares as tiles.
-__device__ __forceinline__ int shares(int ctas, long total) { return int(total < ctas ? total : ctas); }
-__device__ __forceinline__ long share_begin(long c, int n, long total) { return c * total / n; }
-__device__ __forceinline__ int share_of(long t, int n, long total) { return int(((t + 1) * n - 1) / total); }
+// Tiles are dealt in shares of equal size (the last one may be shorter): worker c
+// takes [c * size, (c + 1) * size) of `total`.
+__device__ __forceinline__ int share_size(int workers, int total, int least) {
+  return max((total + workers - 1) / workers, least);
+}
 
 __device__ __forceinline__ long base_slot(const Args& a, int shared, int head, int pair) {
   return (long(shared) * a.hk + head) * a.rows * a.share + pair;
 }
-__device__ __forceinline__ long cta_slot(const Work& w, int cta, int r) {
-  return w.continued + long(cta) * w.item_rows + r;
+// An item's pairs are consecutive and at most item_rows (a power of two), so their
+// low bits tell them apart.
+__device__ __forceinline__ long continued_slot(const Work& w, int worker, int pair) {
+  return w.continued + long(worker) * w.item_rows + (pair & (w.item_rows - 1));
 }
 
-// Thread t's run of items is [t * per, (t + 1) * per); sums[t] becomes the tiles
-// before it. Returns the tiles of one head; CTA 0 leaves every item's first tile
-// for the joining kernel. All THREADS threads of the CTA take part; sums has one
-// entry more.
+// The first tile of every item, in shared memory while there are few items; of more,
+// only of each thread's run [t * per, (t + 1) * per).
+constexpr int kFirsts = 512;
+template <int THREADS>
+struct Deal {
+  int run[THREADS + 1];  // tiles before each thread's run; the last entry: tiles of one head
+  int first[kFirsts + 1];
+};
+
+// Numbers the items' tiles; CTA 0 leaves every item's first tile for the joining
+// kernel. All THREADS threads of the CTA take part. Returns the tiles of one head.
 template <int TK, int THREADS>
-__device__ __forceinline__ int deal(const Args& a, const Work& w, int* sums) {
+__device__ __forceinline__ int deal(const Args& a, const Work& w, Deal<THREADS>& d) {
   const int tid = threadIdx.x, per = (w.n + THREADS - 1) / THREADS;
   const int i0 = min(w.n, tid * per), i1 = min(w.n, i0 + per);
   int mine = 0;
   for (int i = i0; i < i1; ++i) mine += tiles_of<TK>(a, w.items[i]);
-  sums[tid] = mine;
+  d.run[tid] = mine;
   __syncthreads();
   if (tid < 32) {
     int run = 0;
     for (int b = 0; b < THREADS; b += 32) {
-      const int v = sums[b + tid];
+      const int v = d.run[b + tid];
       int x = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (tid >= o) x += y;
       }
-      sums[b + tid] = run + x - v;
+      d.run[b + tid] = run + x - v;
       run += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (tid == 0) sums[THREADS] = run;
+    if (tid == 0) d.run[THREADS] = run;
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
-    int t = sums[tid];
+  if (blockIdx.x == 0 || w.n <= kFirsts) {
+    int t = d.run[tid];
     for (int i = i0; i < i1; ++i) {
-      w.tile0[i] = t;
-      t += tiles_of<TK>(a, w.items[i]);
+      if (w.n <= kFirsts) d.first[i] = t;
+      if (blockIdx.x == 0) w.tile0[i] = t;
+      t += per == 1 ? mine : tiles_of<TK>(a, w.items[i]);
     }
-    if (tid == 0) w.tile0[w.n] = sums[THREADS];
+    if (tid == 0) {
+      if (w.n <= kFirsts) d.first[w.n] = d.run[THREADS];
+      if (blockIdx.x == 0) w.tile0[w.n] = d.run[THREADS];
+    }
   }
-  return sums[THREADS];
+  __syncthreads();
+  return d.run[THREADS];
 }
 
 // The item that holds tile t of a head; `at` becomes its first tile, `n` its tiles.
 template <int TK, int THREADS>
-__device__ __forceinline__ int item_of(const Args& a, const Work& w, const int* sums, int t, int& at, int& n) {
-  int lo = 0, hi = THREADS - 1;  // the last run whose first tile is not past t
+__device__ __forceinline__ int item_of(const Args& a, const Work& w, const Deal<THREADS>& d, int t, int& at, int& n) {
+  const bool few = w.n <= kFirsts;
+  const int* first = few ? d.first : d.run;
+  int lo = 0, hi = (few ? w.n : THREADS) - 1;  // the last whose first tile is not past t
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (sums[mid] <= t) lo = mid;
+    if (first[mid] <= t) lo = mid;
     else hi = mid - 1;
   }
+  at = first[lo];
+  if (few) {
+    n = first[lo + 1] - at;
+    return lo;
+  }
   int i = lo * ((w.n + THREADS - 1) / THREADS);
-  at = sums[lo];
   n = tiles_of<TK>(a, w.items[i]);
   while (at + n <= t) {
     at += n;
     n = tiles_of<TK>(a, w.items[++i]);
   }
   return i;
+}
+
+// The table row that an item's keys are read through, and the end of those that
+// exist; by a whole warp. Shared pages are read through the first sequence that
+// holds all of them, else through the longest (idle slots hold none).
+__device__ __forceinline__ void run_end(const Args& a, const Item& item, int& slot, int& end) {
+  const int lane = threadIdx.x % 32;
+  slot = item.first;
+  if (!item.shared) {
+    end = length_of(a, slot) - item.keys;
+    return;
+  }
+  const int all = item.key0 + item.keys;
+  int best = -1;
+  for (int s = item.first; s < item.first + item.count && best < all; s += 32) {
+    const bool there = s + lane < item.first + item.count;
+    const int c = there ? a.slot_of_seq[s + lane] : 0, len = there ? length_of(a, c) : -1;
+    const unsigned full = __ballot_sync(0xffffffffu, len >= all);
+    int most = len;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const unsigned longest = __ballot_sync(0xffffffffu, len == most);
+    const int from = __ffs(full ? full : longest) - 1;
+    if (full || most > best) {
+      best = __shfl_sync(0xffffffffu, len, from);
+      slot = __shfl_sync(0xffffffffu, c, from);
+    }
+  }
+  end = min(best, all);
 }
 
 template <typename T>

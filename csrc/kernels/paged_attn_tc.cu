@@ -9,10 +9,13 @@
 //   warp 0      finds the pieces, writes their records, loads K and V: a lane a page
 //   warp 1      issues the MMAs, S_t = Q_t K^T and O_t += P_t V (P_t in tensor
 //               memory over the columns of S_t)
-//   warps 2-5   softmax of tile 0, warps 6-9 of tile 1: thread = row. They bring
-//               their row of Q to shared memory at the start of a piece and write its
-//               partial at the end. O is rescaled only when a row's maximum grew by
-//               2^8 or more since the last time; the stale maximum scales P and O alike.
+//   warps 2-9   softmax of tile 0, warps 10-17 of tile 1. Two threads have a row, each
+//               half of the tile's keys; they exchange their maxima by shared memory.
+//               (Exponentials are the bound; two warps a tile and scheduler hide each
+//               other's loads and barriers.) They bring their row of Q to shared memory
+//               at the start of a piece and write its partial at the end. O is rescaled
+//               only when a row's maximum grew by 2^8 or more since the last time; the
+//               stale maximum scales P and O alike.
 // Keys past the end of an item's run are hidden by the mask; their values are
 // cleared in shared memory first, since 0 * NaN is not 0.
 #include <ATen/cuda/CUDAContext.h>
@@ -29,7 +32,8 @@ namespace pa {
 
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 576;
+constexpr int kSoftWarps = 8;  // of one tile
 constexpr int kPieces = 8;  // records; the producer is at most four pieces ahead of the slowest role
 constexpr float kRescale = 8.f;
 
@@ -38,6 +42,7 @@ struct Piece {
   int key0, tiles;   // first key and tiles of the piece
   int end;           // keys of the item's run that exist
   int continued;
+  int final;         // nothing to join: the piece writes the output
 };
 
 template <int D>
@@ -46,6 +51,29 @@ struct Big {
   static constexpr int kTile = kSub * (D / 64);     // Q, K or V tile
   static constexpr int kSmem = 1024 + 6 * kTile;    // Q0, Q1, two K, two V
 };
+
+// One lane of a warp that is whole, and a value that is the same in all its lanes:
+// in forms that the compiler knows as such.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return reinterpret_cast<float2&>(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return reinterpret_cast<float2&>(d);
+}
 
 // bf16 operands have format 1 in bits 7 and 10 of the descriptor, fp16 format 0.
 template <typename T>
@@ -62,24 +90,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = smem + 2 * S::kTile, *sV = smem + 4 * S::kTile;
-  __shared__ int s_sum[kThreads + 1];
+  __shared__ Deal<kThreads> dealt;
   __shared__ Piece pieces[kPieces];
   __shared__ uint64_t piece_full[kPieces], q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clear, s_full[2],
-      p_full[2], o_done[2];
+      p_full[2], o_done[2], both[2][4];  // both: the two warps that share 32 rows
+  __shared__ float s_row[2][2][2][128];  // exchanged between a row's threads: [parity][tile][half][row]
   __shared__ uint32_t tmem_slot;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
   const Work& w = a.work[1];
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPieces; ++i) mbar_init(&piece_full[i], 1);
-    mbar_init(&q_full, 8);
-    mbar_init(&v_clear, 4);
+    mbar_init(&q_full, 2 * kSoftWarps);
+    mbar_init(&v_clear, kSoftWarps);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], kSoftWarps);
+      for (int q = 0; q < 4; ++q) mbar_init(&both[i][q], 2);
       mbar_init(&o_done[i], 1);
     }
     fence_barrier_init();
@@ -87,53 +117,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tm_v);
   }
   if (warp == 1) tmem_alloc(&tmem_slot, 512);
-  const int head_tiles = deal<BK, kThreads>(a, w, s_sum);
+  pdl_trigger();
+  const int head_tiles = deal<BK, kThreads>(a, w, dealt);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;  // S0 @0, S1 @128, O0 @256, O1 @256 + D
-  const long total = long(head_tiles) * a.hk;
-  const int n_shares = shares(w.ctas, total);
-  const bool busy = int(blockIdx.x) < n_shares;
-  const long t_begin = busy ? share_begin(blockIdx.x, n_shares, total) : 0;
-  const int n_tiles = busy ? int(share_begin(blockIdx.x + 1, n_shares, total) - t_begin) : 0;
+  const uint32_t tmem = uniform(tmem_slot);  // S0 @0, S1 @128, O0 @256, O1 @256 + D
+  const int total = head_tiles * a.hk, size = share_size(w.workers, total, w.least);
+  const int t_begin = blockIdx.x * size, n_tiles = uniform(min(total - t_begin, size));  // none: n_tiles <= 0
 
   if (warp == 0) {
     const int box_rows = min(a.page, BK);
     int it = 0;  // tiles loaded
     bool ok = true;
     for (int p = 0; it < n_tiles && ok; ++p) {
-      const long t = t_begin + it;
+      const int t = t_begin + it, tt = t % head_tiles;
       int at, n;
-      const int tt = int(t % head_tiles);
-      const int i = item_of<BK, kThreads>(a, w, s_sum, tt, at, n);
+      const int i = item_of<BK, kThreads>(a, w, dealt, tt, at, n);
       const Item item = w.items[i];
-      int slot = item.first, end;
-      if (item.shared) {
-        // Read through the first sequence that holds all of the shared tokens, else
-        // through the longest (idle slots hold none).
-        int best = -1;
-        for (int s = item.first; s < item.first + item.count && best < item.key0 + item.keys; s += 32) {
-          const bool there = s + lane < item.first + item.count;
-          const int c = there ? a.slot_of_seq[s + lane] : 0, len = there ? length_of(a, c) : -1;
-          const unsigned full = __ballot_sync(0xffffffffu, len >= item.key0 + item.keys);
-          int most = len;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const unsigned longest = __ballot_sync(0xffffffffu, len == most);
-          const int from = __ffs(full ? full : longest) - 1;
-          if (full || most > best) {
-            best = __shfl_sync(0xffffffffu, len, from);
-            slot = __shfl_sync(0xffffffffu, c, from);
-          }
-        }
-        end = min(best, item.key0 + item.keys);
-      } else {
-        end = length_of(a, slot) - item.keys;
-      }
-      const int tiles = min(n - (tt - at), n_tiles - it), key0 = item.key0 + (tt - at) * BK, head = int(t / head_tiles);
+      int slot, end;
+      run_end(a, item, slot, end);
+      const int tiles = min(n - (tt - at), n_tiles - it), key0 = item.key0 + (tt - at) * BK, head = t / head_tiles;
       if (lane == 0) {
-        pieces[p % kPieces] = Piece{item.row0, item.rows, head, item.shared, key0, tiles, end, tt != at};
+        pieces[p % kPieces] = Piece{item.row0, item.rows, head, item.shared, key0, tiles, end, tt != at,
+                                   item.alone && tiles == n};
         mbar_arrive(&piece_full[p % kPieces]);
       }
       auto page_of = [&](int j) {  // of this lane's box of tile j of the piece
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b = it & 1, k0 = key0 + j * BK;
         const int boxes = k0 < end ? (min(end - k0, BK) + box_rows - 1) / box_rows : 0;
         const int row = head * a.page + (k0 + lane * box_rows) % a.page;
-        ok = mbar_wait(&k_empty[b], ((it >> 1) & 1) ^ 1, kErrTimeoutProducer, a.err);
+        ok = wait(&k_empty[b], ((it >> 1) & 1) ^ 1, kErrTimeoutProducer, a.err);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_arrive_expect_tx(&k_full[b], boxes * box_rows * D * 2);
         __syncwarp();
@@ -160,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
             tma_load_3d(sK + b * S::kTile + c * S::kSub + lane * box_rows * 128, &tm_k, &k_full[b], c * 64, row, page);
-        ok = mbar_wait(&v_empty[b], ((it >> 1) & 1) ^ 1, kErrTimeoutProducer, a.err);
+        ok = wait(&v_empty[b], ((it >> 1) & 1) ^ 1, kErrTimeoutProducer, a.err);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_arrive_expect_tx(&v_full[b], boxes * box_rows * D * 2);
         __syncwarp();
@@ -173,81 +180,107 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc<T>(128, BK, false), id_o = idesc<T>(128, D, true);
-      uint32_t c_p[2] = {0, 0}, c_clear = 0;  // phases of p_full and v_clear
-      int it = 0;
-      bool ok = true;
-      auto issue_s = [&](int t, int b) {
-        const uint32_t q = smem_u32(sQ + t * S::kTile), k = smem_u32(sK + b * S::kTile);
+    // The whole warp walks the loop and one lane issues: descriptors and phases stay
+    // in uniform registers, which the MMA instruction reads. With the loop itself
+    // on one lane every operand was moved there first, 80 cycles an MMA, and the
+    // issue was the bound.
+    constexpr uint32_t id_s = idesc<T>(128, BK, false), id_o = idesc<T>(128, D, true);
+    const bool leader = elect_one();
+    const uint64_t d_q = sw128_desc(smem_u32(sQ), 16, 1024), d_k = sw128_desc(smem_u32(sK), 16, 1024),
+                   d_v = sw128_desc(smem_u32(sV), S::kSub, 1024);
+    uint32_t c_p0 = 0, c_p1 = 0, c_clear = 0;  // phases of p_full and v_clear
+    int it = 0;
+    bool ok = true;
+    auto issue_s = [&](int t, int b) {
+      const uint64_t q = desc_advance(d_q, t * S::kTile), k = desc_advance(d_k, b * S::kTile);
+      if (leader) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * S::kSub + (kk & 3) * 32;
-          umma_bf16(tmem + t * BK, sw128_desc(q + off, 16, 1024), sw128_desc(k + off, 16, 1024), id_s,
-                    kk > 0 ? 1u : 0u);
+          umma_bf16(tmem + t * BK, desc_advance(q, off), desc_advance(k, off), id_s, kk > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[t]);
-      };
-      auto issue_pv = [&](int t, int b, bool first) {
-        const uint32_t v = smem_u32(sV + b * S::kTile);
+      }
+      __syncwarp();
+    };
+    auto issue_pv = [&](int t, int b, bool first) {
+      const uint64_t v = desc_advance(d_v, b * S::kTile);
+      const uint32_t more = first ? 0u : 1u;
+      if (leader) {
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk)
-          umma_bf16_ts(tmem + 256 + t * D, tmem + t * BK + 8 * kk, sw128_desc(v + kk * 2048, S::kSub, 1024), id_o,
-                       (!first || kk > 0) ? 1u : 0u);
+          umma_bf16_ts(tmem + 256 + t * D, tmem + t * BK + 8 * kk, desc_advance(v, kk * 2048), id_o,
+                       kk > 0 ? 1u : more);
         umma_commit(&o_done[t]);
-      };
-      auto wait_p = [&](int t) {
-        const bool r = mbar_wait(&p_full[t], c_p[t], kErrTimeoutMma, a.err);
-        c_p[t] ^= 1;
+      }
+      __syncwarp();
+    };
+    auto release = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    for (int p = 0; it < n_tiles && ok; ++p) {
+      if (!(ok = wait(&piece_full[p % kPieces], (p / kPieces) & 1, kErrTimeoutMma, a.err))) break;
+      const int rows = uniform(pieces[p % kPieces].rows), tiles = uniform(pieces[p % kPieces].tiles);
+      const int keys = uniform(pieces[p % kPieces].end - pieces[p % kPieces].key0);
+      const bool two = rows > 128;
+      if (!(ok = wait(&q_full, p & 1, kErrTimeoutMma, a.err))) break;
+      if (!(ok = wait(&k_full[it & 1], (it >> 1) & 1, kErrTimeoutMma, a.err))) break;
+      tc_fence_after();
+      issue_s(0, it & 1);
+      if (two) issue_s(1, it & 1);
+      release(&k_empty[it & 1]);
+      for (int j = 0; j < tiles; ++j, ++it) {
+        const bool next = j + 1 < tiles;
+        const int b = it & 1, nb = b ^ 1;
+        if (!(ok = wait(&v_full[b], (it >> 1) & 1, kErrTimeoutMma, a.err))) break;
+        if (keys - j * BK < BK) {
+          if (!(ok = wait(&v_clear, c_clear, kErrTimeoutMma, a.err))) break;
+          c_clear ^= 1;
+        }
+        if (!(ok = wait(&p_full[0], c_p0, kErrTimeoutMma, a.err))) break;
+        c_p0 ^= 1;
         tc_fence_after();
-        return r;
-      };
-      for (int p = 0; it < n_tiles && ok; ++p) {
-        if (!mbar_wait(&piece_full[p % kPieces], (p / kPieces) & 1, kErrTimeoutMma, a.err)) break;
-        const Piece pc = pieces[p % kPieces];
-        const bool two = pc.rows > 128;
-        if (!mbar_wait(&q_full, p & 1, kErrTimeoutMma, a.err)) break;
-        if (!mbar_wait(&k_full[it & 1], (it >> 1) & 1, kErrTimeoutMma, a.err)) break;
-        tc_fence_after();
-        issue_s(0, it & 1);
-        if (two) issue_s(1, it & 1);
-        umma_commit(&k_empty[it & 1]);
-        for (int j = 0; j < pc.tiles && ok; ++j, ++it) {
-          const bool next = j + 1 < pc.tiles;
-          const int b = it & 1, nb = b ^ 1;
-          ok = mbar_wait(&v_full[b], (it >> 1) & 1, kErrTimeoutMma, a.err);
-          if (pc.end - pc.key0 - j * BK < BK && ok) {
-            ok = mbar_wait(&v_clear, c_clear, kErrTimeoutMma, a.err);
-            c_clear ^= 1;
-          }
-          if (!ok || !(ok = wait_p(0))) break;
-          issue_pv(0, b, j == 0);
-          if (next) {
-            if (!(ok = mbar_wait(&k_full[nb], ((it + 1) >> 1) & 1, kErrTimeoutMma, a.err))) break;
-            tc_fence_after();
-            issue_s(0, nb);
-          }
-          if (two) {
-            if (!(ok = wait_p(1))) break;
-            issue_pv(1, b, j == 0);
-          }
-          umma_commit(&v_empty[b]);
-          if (next) {
-            if (two) issue_s(1, nb);
-            umma_commit(&k_empty[nb]);
-          }
+        issue_pv(0, b, j == 0);
+        if (next) {
+          if (!(ok = wait(&k_full[nb], ((it + 1) >> 1) & 1, kErrTimeoutMma, a.err))) break;
+          tc_fence_after();
+          issue_s(0, nb);
+        }
+        if (two) {
+          if (!(ok = wait(&p_full[1], c_p1, kErrTimeoutMma, a.err))) break;
+          c_p1 ^= 1;
+          tc_fence_after();
+          issue_pv(1, b, j == 0);
+        }
+        release(&v_empty[b]);
+        if (next) {
+          if (two) issue_s(1, nb);
+          release(&k_empty[nb]);
         }
       }
     }
   } else {
-    const int t = (warp - 2) / 4, quarter = warp & 3, r = quarter * 32 + lane;
+    constexpr int HK = BK / 2, HD = D / 2;  // of a thread: keys of a tile, columns of O
+    const int t = (warp - 2) / kSoftWarps, half = (warp - 2) / 4 % 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const uint32_t t_s = tmem + lanes + t * BK, t_o = tmem + lanes + 256 + t * D;
-    uint32_t c_s = 0, c_o = 0;  // phases of s_full and o_done
+    const uint32_t t_s = tmem + lanes + t * BK, t_o = tmem + lanes + 256 + t * D + half * HD;
+    uint32_t c_s = 0, c_o = 0, c_b = 0;  // phases of s_full, o_done and both
     int it = 0;
     bool ok = true;
+    // The other thread's value of this row.
+    auto exchange = [&](float x, float& other) {
+      float(&slot)[2][128] = s_row[c_b][t];
+      slot[half][r] = x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&both[t][quarter]);
+      const bool done = wait(&both[t][quarter], c_b, kErrTimeoutEpilogue, a.err);
+      c_b ^= 1;
+      other = slot[half ^ 1][r];
+      return done;
+    };
     for (int p = 0; it < n_tiles && ok; ++p) {
-      if (!mbar_wait(&piece_full[p % kPieces], (p / kPieces) & 1, kErrTimeoutEpilogue, a.err)) break;
+      if (!wait(&piece_full[p % kPieces], (p / kPieces) & 1, kErrTimeoutEpilogue, a.err)) break;
       const Piece pc = pieces[p % kPieces];
       const int pair = pc.row0 + t * 128 + r;
       const bool active = pc.rows > t * 128, mine = t * 128 + r < pc.rows;
@@ -262,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Chunk c of row r lies at c ^ (r & 7), the swizzle that the tensor core reads.
         const bool wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
+        for (int i = 0; i < HD / 8; ++i) {
+          const int c = half * (HD / 8) + i;
           uint4 x = make_uint4(0, 0, 0, 0);
           if (mine && wide) {
             x = *reinterpret_cast<const uint4*>(src + c * 8);
@@ -274,109 +308,135 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_proxy_async();
       }
-      // All eight warps arrive for every piece, each once the last piece's arrivals
-      // are complete: nobody is counted twice and nobody falls a piece behind.
-      if (p > 0 && !mbar_wait(&q_full, (p - 1) & 1, kErrTimeoutEpilogue, a.err)) break;
+      // All warps arrive for every piece, each once the last piece's arrivals are
+      // complete: nobody is counted twice and nobody falls a piece behind.
+      if (p > 0 && !wait(&q_full, (p - 1) & 1, kErrTimeoutEpilogue, a.err)) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
       if (!active) {
         it += pc.tiles;
         continue;
       }
-      float m_used = -INFINITY, l = 0.f;
+      float m_used = -INFINITY, l = 0.f;  // l: of this thread's keys
       for (int j = 0; j < pc.tiles && ok; ++j, ++it) {
         const int k0 = pc.key0 + j * BK, valid = pc.end - k0;
         if (t == 0 && valid < BK) {
           // Thread = key: clear the values of keys that do not exist.
-          if (!(ok = mbar_wait(&v_full[it & 1], (it >> 1) & 1, kErrTimeoutEpilogue, a.err))) break;
+          if (!(ok = wait(&v_full[it & 1], (it >> 1) & 1, kErrTimeoutEpilogue, a.err))) break;
           if (r >= valid)
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c)
+            for (int i = 0; i < HD / 8; ++i) {
+              const int c = half * (HD / 8) + i;
               *reinterpret_cast<uint4*>(sV + (it & 1) * S::kTile + (c / 8) * S::kSub + r * 128 + (c & 7) * 16) =
                   make_uint4(0, 0, 0, 0);
+            }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&v_clear);
         }
-        if (!(ok = mbar_wait(&s_full[t], c_s, kErrTimeoutEpilogue, a.err))) break;
+        if (!(ok = wait(&s_full[t], c_s, kErrTimeoutEpilogue, a.err))) break;
         c_s ^= 1;
         tc_fence_after();
-        float sv[BK];
-        tmem_ld_32x64(t_s, *reinterpret_cast<float(*)[64]>(sv));
-        tmem_ld_32x64(t_s + 64, *reinterpret_cast<float(*)[64]>(sv + 64));
-        const int see = min(lim - k0, valid);
-        if (__any_sync(0xffffffffu, see < BK)) {
+        float2 sv[HK / 2];
+        tmem_ld_32x64(t_s + half * HK, *reinterpret_cast<float(*)[64]>(sv));
+        const int see = min(lim - k0, valid) - half * HK;
+        if (__any_sync(0xffffffffu, see < HK)) {
 #pragma unroll
-          for (int i = 0; i < BK; ++i)
-            if (i >= see) sv[i] = -INFINITY;
+          for (int i = 0; i < HK / 2; ++i) {
+            if (2 * i >= see) sv[i].x = -INFINITY;
+            if (2 * i + 1 >= see) sv[i].y = -INFINITY;
+          }
         }
-        float mx8[8];
+        float mx4[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = sv[k];
+        for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(sv[k].x, sv[k].y);
 #pragma unroll
-        for (int i = 8; i < BK; i += 8)
+        for (int i = 4; i < HK / 2; i += 4)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], sv[i + k]);
-        const float mx = a.sl2 * fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                       fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+          for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(mx4[k], fmaxf(sv[i + k].x, sv[i + k].y));
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), mx_other;
+        // Both threads have read their scores once this is done, so either may store P over them.
+        tc_fence_before();
+        if (!(ok = exchange(mx, mx_other))) break;
+        tc_fence_after();
+        mx = a.sl2 * fmaxf(mx, mx_other);
+        const bool grow = mx > m_used + kRescale || (m_used == -INFINITY && mx > -INFINITY);
         // The P V before this one must be done before P is rewritten or O rescaled.
         if (j > 0) {
-          if (!(ok = mbar_wait(&o_done[t], c_o, kErrTimeoutEpilogue, a.err))) break;
+          if (!(ok = wait(&o_done[t], c_o, kErrTimeoutEpilogue, a.err))) break;
           c_o ^= 1;
           tc_fence_after();
         }
-        const bool grow = mx > m_used + kRescale || (m_used == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
           const float m_new = grow ? mx : m_used;
           const float alpha = grow ? ex2_approx(m_used - m_new) : 1.f;
           if (j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld_32x32(t_o + c * 32, o);
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x16_issue(t_o + c * 16, o);
+              tmem_ld_wait16(o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= alpha;
-              tmem_st_32x32(t_o + c * 32, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x16(t_o + c * 16, o);
             }
           }
           l *= alpha;
           m_used = m_new;
         }
         const float ref = m_used == -INFINITY ? 0.f : m_used;  // a row that has seen no key yet
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 scale2 = make_float2(a.sl2, a.sl2), ref2 = make_float2(-ref, -ref);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < BK / 32; ++c) {
+        for (int c = 0; c < HK / 32; ++c) {
           uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = ex2_approx(fmaf(sv[c * 32 + i], a.sl2, -ref));
-            const float p1 = ex2_approx(fmaf(sv[c * 32 + i + 1], a.sl2, -ref));
-            sum[(i >> 1) & 3] += p0 + p1;
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = fma2(sv[c * 16 + i], scale2, ref2);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum[i & 1] = add2(sum[i & 1], e);
             // P is rounded to the values' type for the tensor core; the sum keeps fp32.
-            pk[i / 2] = pack<T>(p0, p1);
+            pk[i] = pack<T>(e.x, e.y);
           }
-          tmem_st_32x16_issue(t_s + 16 * c, pk);
+          tmem_st_32x16_issue(t_s + half * (HK / 2) + 16 * c, pk);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      if (!ok || !mbar_wait(&o_done[t], c_o, kErrTimeoutEpilogue, a.err)) break;
+      float l_other;
+      if (!ok || !exchange(l, l_other) || !wait(&o_done[t], c_o, kErrTimeoutEpilogue, a.err)) break;
       c_o ^= 1;
+      l += l_other;
       tc_fence_after();
-      const long slot = pc.continued ? cta_slot(w, blockIdx.x, t * 128 + r) : base_slot(a, pc.shared, pc.head, pair);
-      if (mine) a.part_ml[slot] = make_float2(m_used, l);
+      const long slot = pc.continued ? continued_slot(w, blockIdx.x, pair)
+                                     : base_slot(a, pc.shared, pc.head, pair);
+      const int row = mine ? pair / a.share : 0, h = pc.head * a.share + (mine ? pair % a.share : 0);
+      const float inv = inverse(l);
+      T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + half * HD;
+      if (mine && half == 0) {
+        if (!pc.final) a.part_ml[slot] = make_float2(m_used, l);
+        else if (a.lse) a.lse[long(row) * a.hk * a.share + h] = lse_of(m_used, l);
+      }
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        tmem_ld_32x32(t_o + c * 32, o);
-        if (mine)
+      for (int c = 0; c < HD / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld_32x16_issue(t_o + c * 16, o);
+        tmem_ld_wait16(o);
+        if (mine && pc.final) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(a.part_o + slot * D + c * 32 + i) =
-                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 16; i += 2)
+            *reinterpret_cast<uint32_t*>(dst + c * 16 + i) =
+                pack<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+        } else if (mine) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(a.part_o + slot * D + half * HD + c * 16 + i) =
+                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
       }
       tc_fence_before();  // O is read before the next piece's first P V overwrites it
     }
@@ -400,7 +460,7 @@ void launch_big(const CUtensorMap& k, const CUtensorMap& v, const Args& a, cudaS
     return true;
   }();
   (void)configured;
-  paged_attn_tc_kernel<T, D><<<a.work[1].ctas, kThreads, smem, stream>>>(k, v, a);
+  paged_attn_tc_kernel<T, D><<<a.work[1].workers, kThreads, smem, stream>>>(k, v, a);
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "paged_attention launch failed");
 }
 

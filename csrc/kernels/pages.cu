@@ -12,10 +12,11 @@
 // page belongs to one sequence. New pages are the lowest free ones, handed out in
 // the order of the call's list, so every result is defined exactly.
 //
-// Each operator is one launch of a single cluster that rewrites table, lens and
-// refs (into fresh tensors or in place) in phases separated by cluster barriers,
-// and, where rows move, a second launch that copies them from a list of pairs
-// that the first one left in the workspace.
+// Each operator is one launch that rewrites table, lens and refs (into fresh
+// tensors or in place) in phases separated by barriers, and, where rows move, a
+// second launch that copies them from a list of pairs that the first one left in
+// the workspace. The first is bound by its chain of barriers and look-ups: one CTA
+// runs it while the state is small, a cluster of eight when there is much to read.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -23,15 +24,27 @@
 #include <climits>
 
 #include "common.cuh"
+#include "launch.h"
 #include "message.h"
 #include "status.h"
 
 namespace nk {
 namespace {
 
-constexpr int kMetaCtas = 8;        // one portable cluster
 constexpr int kMetaThreads = 1024;
-constexpr int kMetaAll = kMetaCtas * kMetaThreads;
+constexpr int kMetaCtas = 8;  // one portable cluster
+
+// The threads that work on the state: a CTA, or a cluster of C.
+template <int C>
+struct Team {
+  static constexpr int kAll = C * kMetaThreads, kWarps = kAll / 32;
+  __device__ static int cta() { return C == 1 ? 0 : int(cluster_rank()); }
+  __device__ static int gid() { return cta() * kMetaThreads + int(threadIdx.x); }
+  __device__ static void sync() {
+    if constexpr (C == 1) __syncthreads();
+    else cluster_sync();
+  }
+};
 
 struct PageState {
   const int *table_in, *lens_in, *refs_in;
@@ -48,12 +61,24 @@ __device__ __forceinline__ void report(int* err, int code) { atomicCAS(err, 0, c
 
 __device__ __forceinline__ bool copies(const PageState& s) { return s.table != s.table_in; }
 
-// table, lens and refs into the outputs, all threads of the cluster.
-__device__ __forceinline__ void copy_state(const PageState& s, int gid) {
+// table, lens and refs into the outputs, by the whole team.
+template <int C>
+__device__ __forceinline__ void copy_state(const PageState& s) {
   if (!copies(s)) return;
-  for (long i = gid; i < long(s.slots) * s.width; i += kMetaAll) s.table[i] = s.table_in[i];
-  for (int i = gid; i < s.slots; i += kMetaAll) s.lens[i] = s.lens_in[i];
-  for (int i = gid; i < s.pages; i += kMetaAll) s.refs[i] = s.refs_in[i];
+  constexpr int all = Team<C>::kAll, U = 4;
+  const int gid = Team<C>::gid();
+  const long n = long(s.slots) * s.width;
+  for (long i = gid; i < n; i += long(U) * all) {
+    int x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + long(u) * all < n) x[u] = s.table_in[i + long(u) * all];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + long(u) * all < n) s.table[i + long(u) * all] = x[u];
+  }
+  for (int i = gid; i < s.slots; i += all) s.lens[i] = s.lens_in[i];
+  for (int i = gid; i < s.pages; i += all) s.refs[i] = s.refs_in[i];
 }
 
 // Exclusive sum over a CTA's threads; every thread also gets the total.
@@ -82,59 +107,58 @@ __device__ __forceinline__ int cta_scan(int v, int* sm, int& total) {
   return (warp ? sm[warp - 1] : 0) + x - v;
 }
 
-// Thread `gid` of the cluster owns pages [lo, hi). Returns how many pages before
-// lo have refs > 0, and the number of all such pages. One cluster barrier.
-__device__ __forceinline__ int live_before(const int* refs, int pages, int gid, int* sm, int* ws, int& lo, int& hi,
-                                           int& live) {
-  const int span = (pages + kMetaAll - 1) / kMetaAll;
-  lo = min(pages, gid * span);
+// Each thread of the team owns pages [lo, hi). Returns how many pages before lo
+// have refs > 0, and the number of all such pages. One barrier of the team.
+template <int C>
+__device__ __forceinline__ int live_before(const int* refs, int pages, int* sm, int* ws, int& lo, int& hi, int& live) {
+  const int span = (pages + Team<C>::kAll - 1) / Team<C>::kAll;
+  lo = min(pages, Team<C>::gid() * span);
   hi = min(pages, lo + span);
   int mine = 0;
   for (int p = lo; p < hi; ++p) mine += refs[p] > 0;
   int total;
   int before = cta_scan(mine, sm, total);
-  const int cta = int(cluster_rank());
-  if (threadIdx.x == 0) ws[kWsCounts + cta] = total;
-  cluster_sync();
-  live = 0;
-  for (int c = 0; c < kMetaCtas; ++c) {
-    const int n = __ldcg(ws + kWsCounts + c);
-    if (c < cta) before += n;
-    live += n;
+  if (C > 1 && threadIdx.x == 0) ws[kWsCounts + Team<C>::cta()] = total;
+  Team<C>::sync();
+  live = total;
+  if constexpr (C > 1) {
+    live = 0;
+    for (int c = 0; c < C; ++c) {
+      const int n = __ldcg(ws + kWsCounts + c);
+      if (c < Team<C>::cta()) before += n;
+      live += n;
+    }
   }
   return before;
 }
-
-__device__ __forceinline__ int meta_gid() { return int(cluster_rank()) * kMetaThreads + int(threadIdx.x); }
-
-// Sequences are handed to the cluster's warps in turn.
-constexpr int kMetaWarps = kMetaAll / 32;
-__device__ __forceinline__ int meta_warp() { return meta_gid() / 32; }
 
 // ---- fork ----------------------------------------------------------------------
 
 // ws lists: owner (slots); then n each of: free pages, pair sources, pair
 // targets, pair rows, lengths of the children to make (-1: none).
-__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+template <int C>
+__global__ void __launch_bounds__(kMetaThreads)
     fork_meta_kernel(const PageState s, const int* __restrict__ parents, const int* __restrict__ children, int n,
                      int* ws) {
   __shared__ int sm[32];
-  const int gid = meta_gid();
+  using team = Team<C>;
+  const int gid = team::gid();
+  pdl_trigger();
   int *owner = ws + kListAt, *spare = owner + s.slots, *src = spare + n, *dst = src + n, *rows = dst + n,
       *length = rows + n;
-  copy_state(s, gid);
-  for (int i = gid; i < s.slots; i += kMetaAll) owner[i] = INT_MAX;
+  copy_state<C>(s);
+  for (int i = gid; i < s.slots; i += team::kAll) owner[i] = INT_MAX;
   int lo, hi, live;
-  const int before = live_before(s.refs_in, s.pages, gid, sm, ws, lo, hi, live);
+  const int before = live_before<C>(s.refs_in, s.pages, sm, ws, lo, hi, live);
   for (int p = lo, f = lo - before; p < hi && f < n; ++p)
     if (s.refs_in[p] <= 0) spare[f++] = p;
   // A slot that the list names twice goes to its first mention.
-  for (int i = gid; i < n; i += kMetaAll) {
+  for (int i = gid; i < n; i += team::kAll) {
     const int c = children[i];
     if (c >= 0 && c < s.slots) atomicMin(owner + c, i);
   }
-  cluster_sync();
-  if (cluster_rank() == 0) {
+  team::sync();
+  if (team::cta() == 0) {
     // Which children are made, and the page of each that needs one: by one CTA,
     // in the list's order.
     const int span = (n + kMetaThreads - 1) / kMetaThreads;
@@ -164,8 +188,8 @@ __global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads
       }
     }
   }
-  cluster_sync();
-  for (int i = meta_warp(); i < n; i += kMetaWarps) {
+  team::sync();
+  for (int i = gid / 32; i < n; i += team::kWarps) {
     const int len = __ldcg(length + i), lane = threadIdx.x % 32;
     if (len < 0) continue;
     const int* from = s.table_in + long(parents[i]) * s.width;
@@ -189,18 +213,21 @@ __global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads
 // ---- grow ----------------------------------------------------------------------
 
 // ws list: free pages (pages).
-__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+template <int C>
+__global__ void __launch_bounds__(kMetaThreads)
     grow_meta_kernel(const PageState s, const int* __restrict__ add, int* ws) {
   __shared__ int sm[32];
-  const int gid = meta_gid();
+  using team = Team<C>;
+  const int gid = team::gid();
+  pdl_trigger();
   int* spare = ws + kListAt;
-  copy_state(s, gid);
+  copy_state<C>(s);
   int lo, hi, live;
-  const int before = live_before(s.refs_in, s.pages, gid, sm, ws, lo, hi, live);
+  const int before = live_before<C>(s.refs_in, s.pages, sm, ws, lo, hi, live);
   for (int p = lo, f = lo - before; p < hi; ++p)
     if (s.refs_in[p] <= 0) spare[f++] = p;
-  cluster_sync();
-  if (cluster_rank() != 0) return;
+  team::sync();
+  if (team::cta() != 0) return;
   const int span = (s.slots + kMetaThreads - 1) / kMetaThreads;
   const int i0 = min(s.slots, int(threadIdx.x) * span), i1 = min(s.slots, i0 + span);
   auto need = [&](int i, int& len, int& have) {  // pages that slot i lacks; -1: it cannot be grown
@@ -233,11 +260,14 @@ __global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads
 
 // ---- free ----------------------------------------------------------------------
 
-__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+template <int C>
+__global__ void __launch_bounds__(kMetaThreads)
     free_meta_kernel(const PageState s, const int* __restrict__ seqs, int n) {
-  copy_state(s, meta_gid());
-  cluster_sync();
-  for (int i = meta_warp(); i < n; i += kMetaWarps) {
+  using team = Team<C>;
+  const int gid = team::gid();
+  copy_state<C>(s);
+  team::sync();
+  for (int i = gid / 32; i < n; i += team::kWarps) {
     const int slot = seqs[i], lane = threadIdx.x % 32;
     if (slot < 0 || slot >= s.slots) {
       if (lane == 0) report(s.err, kErrBounds);
@@ -261,14 +291,17 @@ __global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads
 // i-th of the others (ascending) moves to the i-th free page below L.
 // ws lists (pages each): pair sources, pair targets, sources from the last one
 // down, new number of each page.
-__global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads)
+template <int C>
+__global__ void __launch_bounds__(kMetaThreads)
     compact_meta_kernel(const PageState s, int* ws) {
   __shared__ int sm[32];
-  const int gid = meta_gid();
+  using team = Team<C>;
+  const int gid = team::gid();
+  pdl_trigger();
   int *src = ws + kListAt, *dst = src + s.pages, *down = dst + s.pages, *to = down + s.pages;
-  copy_state(s, gid);
+  copy_state<C>(s);
   int lo, hi, live;
-  int r = live_before(s.refs_in, s.pages, gid, sm, ws, lo, hi, live);
+  int r = live_before<C>(s.refs_in, s.pages, sm, ws, lo, hi, live);
   if (gid == 0 && live == s.pages) ws[kWsPairs] = 0;
   for (int p = lo; p < hi; ++p) {
     const bool used = s.refs_in[p] > 0;
@@ -278,17 +311,17 @@ __global__ void __cluster_dims__(kMetaCtas, 1, 1) __launch_bounds__(kMetaThreads
     if (used && p >= live) down[live - 1 - r] = p;
     r += used;
   }
-  cluster_sync();
+  team::sync();
   const int pairs = __ldcg(ws + kWsPairs);
-  for (int i = gid; i < pairs; i += kMetaAll) {
+  for (int i = gid; i < pairs; i += team::kAll) {
     const int from = __ldcg(down + pairs - 1 - i), t = __ldcg(dst + i);
     src[i] = from;
     to[from] = t;
     s.refs[t] = s.refs_in[from];
     s.refs[from] = 0;
   }
-  cluster_sync();
-  for (long i = gid; i < long(s.slots) * s.width; i += kMetaAll) {
+  team::sync();
+  for (long i = gid; i < long(s.slots) * s.width; i += team::kAll) {
     const int q = s.table_in[i];
     if (q >= 0 && q < s.pages) s.table[i] = __ldcg(to + q);
   }
@@ -310,6 +343,7 @@ constexpr int kCopyThreads = 256;
 // A warp copies the rows of one (pair, layer, k or v, head): up to 2 KB of
 // loads in flight, neighbouring warps on neighbouring heads of a page.
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs a) {
+  pdl_wait();  // the list may be the state kernel's
   const int lane = threadIdx.x % 32;
   const long warps = long(gridDim.x) * (kCopyThreads / 32);
   const int n = a.count ? min(*a.count, a.n) : a.n;
@@ -403,9 +437,30 @@ CopyArgs pools_of(const torch::Tensor& k, const torch::Tensor& v, const torch::T
 void launch_copy(const CopyArgs& a) {
   const int64_t units = int64_t(a.n) * a.layers * 2 * a.heads;
   if (units == 0) return;
-  const int64_t blocks = std::min<int64_t>((units + kCopyThreads / 32 - 1) / (kCopyThreads / 32), 148 * 8);
-  copy_pages_kernel<<<unsigned(blocks), kCopyThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "copy_pages launch failed");
+  // Four rounds of CTAs, so that one that starts late (its SM still held by the state
+  // kernel) does not end late: with one round of longer CTAs, 252 forks took 185 us
+  // instead of 162.
+  const int64_t blocks = std::min<int64_t>((units + kCopyThreads / 32 - 1) / (kCopyThreads / 32), 148 * 32);
+  TORCH_CHECK(launch_early(copy_pages_kernel, dim3(unsigned(blocks)), dim3(kCopyThreads), 0,
+                           at::cuda::getCurrentCUDAStream(), a) == cudaSuccess, "copy_pages launch failed");
+}
+
+// One CTA while each of its threads has a few entries of the state to read, else a
+// cluster: 256 slots of 32 pages take 7 us on one CTA and 14 us on eight.
+template <typename... KArgs, typename... Args>
+void launch_team(const PageState& s, const char* op, void (*one)(KArgs...), void (*eight)(KArgs...), Args... args) {
+  const bool small = int64_t(s.slots) * s.width + s.slots + s.pages <= 32 * kMetaThreads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(small ? 1 : kMetaCtas);
+  cfg.blockDim = dim3(kMetaThreads);
+  cfg.stream = at::cuda::getCurrentCUDAStream();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = small ? 1 : kMetaCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TORCH_CHECK(cudaLaunchKernelEx(&cfg, small ? one : eight, s, args...) == cudaSuccess, op, " launch failed");
 }
 
 torch::Tensor workspace(const torch::Tensor& like, int64_t ints) {
@@ -427,9 +482,8 @@ void pages_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Te
   const at::cuda::CUDAGuard guard(table.device());
   auto ws = workspace(table, s.slots + 5 * int64_t(n));
   int* w = ws.data_ptr<int>();
-  fork_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
-      s, parents.data_ptr<int>(), children.data_ptr<int>(), n, w);
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fork_pages launch failed");
+  launch_team(s, "fork_pages", fork_meta_kernel<1>, fork_meta_kernel<kMetaCtas>, parents.data_ptr<int>(),
+              children.data_ptr<int>(), n, w);
   c.src = w + kListAt + s.slots + n;
   c.dst = c.src + n;
   c.rows = c.dst + n;
@@ -444,9 +498,8 @@ void pages_grow(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, tor
   TORCH_CHECK(add.sizes() == lens.sizes(), "grow_pages: add must have one entry for each slot");
   const at::cuda::CUDAGuard guard(table.device());
   auto ws = workspace(table, s.pages);
-  grow_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(s, add.data_ptr<int>(),
-                                                                                     ws.data_ptr<int>());
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "grow_pages launch failed");
+  launch_team(s, "grow_pages", grow_meta_kernel<1>, grow_meta_kernel<kMetaCtas>, add.data_ptr<int>(),
+              ws.data_ptr<int>());
 }
 
 void pages_free(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor seqs,
@@ -455,9 +508,8 @@ void pages_free(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, tor
   check_int_vec(seqs, "free_pages: seqs", table);
   TORCH_CHECK(seqs.dim() == 1, "free_pages: seqs must be a vector");
   const at::cuda::CUDAGuard guard(table.device());
-  free_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(s, seqs.data_ptr<int>(),
-                                                                                     int(seqs.size(0)));
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "free_pages launch failed");
+  launch_team(s, "free_pages", free_meta_kernel<1>, free_meta_kernel<kMetaCtas>, seqs.data_ptr<int>(),
+              int(seqs.size(0)));
 }
 
 void pages_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
@@ -468,8 +520,7 @@ void pages_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch:
   const at::cuda::CUDAGuard guard(table.device());
   auto ws = workspace(table, 4 * int64_t(s.pages));
   int* w = ws.data_ptr<int>();
-  compact_meta_kernel<<<kMetaCtas, kMetaThreads, 0, at::cuda::getCurrentCUDAStream()>>>(s, w);
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "compact_pages launch failed");
+  launch_team(s, "compact_pages", compact_meta_kernel<1>, compact_meta_kernel<kMetaCtas>, w);
   c.src = w + kListAt;
   c.dst = c.src + s.pages;
   c.count = w + kWsPairs;

@@ -74,9 +74,9 @@ def copy_pages(k, v, src, dst) -> None:
 
 
 # (row, query head) pairs of an item, as in csrc/kernels/paged_attn.cuh: up to
-# SMALL_ROWS on mma.sync with the keys split over the warps, up to ITEM_ROWS there
-# with the rows split, more on tcgen05, where 128 rows are one tile.
-SMALL_ROWS, ITEM_ROWS, BIG_ROWS, BIG = 16, 64, 256, 1 << 30
+# SMALL_ROWS on mma.sync, up to BIG_ROWS (two tiles of 128) on tcgen05.
+SMALL_ROWS, TILE_ROWS, BIG_ROWS, BIG = 16, 128, 256, 1 << 30
+APART, BIG_FROM = 1.25, 64
 
 
 class PrefixPlan:
@@ -114,26 +114,31 @@ class PrefixPlan:
         back = start[seq + 1] - 1 - np.arange(self.rows)
         lists, of_pair = ([], []), np.full((2, self.rows * share), -1, np.int64)
 
-        def add(shared, first, count, row0, row1, key0, keys):
+        def add(shared, first, count, row0, row1, key0, keys, alone=0):
             pairs = (row1 - row0) * share
-            big = int(pairs > ITEM_ROWS)
-            items, most = lists[big], BIG_ROWS if big else ITEM_ROWS
+            big = int(pairs > BIG_FROM)
+            items, most = lists[big], (SMALL_ROWS, BIG_ROWS)[big]
             for r in range(0, pairs, most):
                 n = min(most, pairs - r)
                 p0 = row0 * share + r
                 of_pair[shared, p0:p0 + n] = len(items) + BIG * big
                 after = keys if shared else back[(p0 + n - 1) // share]
-                items.append((shared, first, count, p0, n, key0, after, int(pairs <= SMALL_ROWS)))
+                items.append((shared, first, count, p0, n, key0, after, alone))
 
         at = 0
         own_from = np.zeros(n_seq, np.int64)
         for n, shared in groups:
-            if n > 1 and shared > 0:  # one sequence has nothing to share
+            # Rows of several sequences fill the tiles of the shared keys better than
+            # each sequence's own would; where they barely do (prompts of many tokens),
+            # one run over all keys saves the joining of two.
+            pairs = t[at:at + n] * share
+            apart, together = (-(-pairs // TILE_ROWS)).sum(), -(-pairs.sum() // TILE_ROWS)
+            if n > 1 and shared > 0 and apart > APART * together:
                 add(1, at, n, start[at], start[at + n], 0, shared)
                 own_from[at:at + n] = shared
             at += n
         for s in range(n_seq):
-            add(0, slot[s], 1, start[s], start[s + 1], own_from[s], 0)
+            add(0, slot[s], 1, start[s], start[s + 1], own_from[s], 0, int(own_from[s] == 0))
 
         def dev(x):
             return torch.as_tensor(np.ascontiguousarray(x), dtype=torch.int32).to(device)

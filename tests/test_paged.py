@@ -602,9 +602,9 @@ def test_plan_items_cpu():
     plan = paged.PrefixPlan([(1, 64), (3, 32), (2, 0)], [3, 40, 1, 0, 2, 5], n_head=6, n_kv_head=2, head_dim=64,
                             page=32, table_width=8, device="cpu")
     seen = {0: [0] * (51 * 3), 1: [0] * (51 * 3)}
-    for list_, most, mark in ((plan.items, 64, 0), (plan.big_items, 256, paged.BIG)):
-        for i, (shared, first, count, row0, rows, key0, keys, small) in enumerate(list_.tolist()):
-            assert 0 < rows <= (16 if small else most)
+    for list_, most, mark in ((plan.items, 16, 0), (plan.big_items, 256, paged.BIG)):
+        for i, (shared, first, count, row0, rows, *_) in enumerate(list_.tolist()):
+            assert 0 < rows <= most
             for p in range(row0, row0 + rows):
                 seen[shared][p] += 1
                 assert (plan.shared_item if shared else plan.own_item)[p] == i + mark
