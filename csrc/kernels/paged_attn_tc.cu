@@ -293,18 +293,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           src = static_cast<const T*>(a.q) + row * a.q_row + (pc.head * a.share + h) * a.q_head;
         }
         // Chunk c of row r lies at c ^ (r & 7), the swizzle that the tensor core reads.
-        const bool wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+        // All of the row's loads are issued before the first store waits for one.
+        const int c0 = half * (HD / 8);
+        uint4 x[HD / 8];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) x[i] = make_uint4(0, 0, 0, 0);
+        if (mine && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) x[i] = reinterpret_cast<const uint4*>(src)[c0 + i];
+        } else if (mine) {
+          const uint32_t* s = reinterpret_cast<const uint32_t*>(src) + c0 * 4;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) x[i] = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+        }
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) {
-          const int c = half * (HD / 8) + i;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (mine && wide) {
-            x = *reinterpret_cast<const uint4*>(src + c * 8);
-          } else if (mine) {
-            const uint32_t* s = reinterpret_cast<const uint32_t*>(src + c * 8);
-            x = make_uint4(s[0], s[1], s[2], s[3]);
-          }
-          *reinterpret_cast<uint4*>(sQ + t * S::kTile + (c / 8) * S::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+          const int c = c0 + i;
+          *reinterpret_cast<uint4*>(sQ + t * S::kTile + (c / 8) * S::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
         }
         fence_proxy_async();
       }
@@ -412,32 +417,57 @@ __global__ void __launch_bounds__(kThreads, 1)
       c_o ^= 1;
       l += l_other;
       tc_fence_after();
-      const long slot = pc.continued ? continued_slot(w, blockIdx.x, pair)
-                                     : base_slot(a, pc.shared, pc.head, pair);
-      const int row = mine ? pair / a.share : 0, h = pc.head * a.share + (mine ? pair % a.share : 0);
+      // A warp's 32 rows go out through its own part of the Q tile (which no MMA
+      // reads any more), C columns at a time: written a row a thread, read as runs of
+      // a row, so that the stores to memory are whole lines. Row by row from the
+      // registers, a piece's write-out took 6 us.
+      constexpr int C = D / 4, V = C / 4;  // V: 16-byte vectors of a row's run
+      uint8_t* stage = sQ + t * S::kTile + (D == 128 ? half * S::kSub + quarter * 4096 : quarter * 4096 + half * 2048);
       const float inv = inverse(l);
-      T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + half * HD;
+      const int hq = a.hk * a.share;
       if (mine && half == 0) {
-        if (!pc.final) a.part_ml[slot] = make_float2(m_used, l);
-        else if (a.lse) a.lse[long(row) * a.hk * a.share + h] = lse_of(m_used, l);
+        if (!pc.final)
+          a.part_ml[pc.continued ? continued_slot(w, blockIdx.x, pair) : base_slot(a, pc.shared, pc.head, pair)] =
+              make_float2(m_used, l);
+        else if (a.lse)
+          a.lse[long(pair / a.share) * hq + pc.head * a.share + pair % a.share] = lse_of(m_used, l);
       }
 #pragma unroll 1
-      for (int c = 0; c < HD / 16; ++c) {
-        uint32_t o[16];
-        tmem_ld_32x16_issue(t_o + c * 16, o);
-        tmem_ld_wait16(o);
-        if (mine && pc.final) {
+      for (int c = 0; c < HD / C; ++c) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 2)
-            *reinterpret_cast<uint32_t*>(dst + c * 16 + i) =
-                pack<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-        } else if (mine) {
+        for (int e = 0; e < C / 16; ++e) {
+          uint32_t o[16];
+          tmem_ld_32x16_issue(t_o + c * C + e * 16, o);
+          tmem_ld_wait16(o);
+          const float f = pc.final ? inv : 1.f;
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint4*>(a.part_o + slot * D + half * HD + c * 16 + i) =
-                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(stage + lane * (C * 4) + (((e * 4 + i) ^ (lane % V)) << 4)) =
+                make_float4(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f,
+                            __uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int rr = i * (32 / V) + lane / V, v = lane % V;  // row of the warp, vector of its run
+          const int row_of = t * 128 + quarter * 32 + rr, pr = pc.row0 + row_of, col = half * HD + c * C + v * 4;
+          if (row_of >= pc.rows) continue;
+          const float4 x = *reinterpret_cast<const float4*>(stage + rr * (C * 4) + ((v ^ (rr % V)) << 4));
+          if (pc.final) {
+            T* dst = static_cast<T*>(a.out) + (pr / a.share) * a.out_row +
+                     (pc.head * a.share + pr % a.share) * a.out_head + col;
+            reinterpret_cast<uint32_t*>(dst)[0] = pack<T>(x.x, x.y);
+            reinterpret_cast<uint32_t*>(dst)[1] = pack<T>(x.z, x.w);
+          } else {
+            const long slot = pc.continued ? continued_slot(w, blockIdx.x, pr) : base_slot(a, pc.shared, pc.head, pr);
+            *reinterpret_cast<float4*>(a.part_o + slot * D + col) = x;
+          }
+        }
+        __syncwarp();
       }
+      // The other warp of these rows has left the Q tile's part, too, before either
+      // brings new rows of Q there.
+      if (!(ok = exchange(0.f, l_other))) break;
       tc_fence_before();  // O is read before the next piece's first P V overwrites it
     }
   }
