@@ -149,30 +149,29 @@ __device__ __forceinline__ void step(Acc<D>& acc, const uint32_t (&qf)[D / 16][4
   }
 }
 
-// A worker's place in its share: a piece is the part of an item that lies in it.
+// The part of an item that lies in a worker's share.
 struct Piece {
-  int left;  // tiles of the share that come after the piece
-  int head, index, tiles, key0, end, slot;  // end: keys of the item's run that exist
+  int head, units, tiles, key0, end, slot;  // end: keys of the item's run that exist
   bool continued, whole;
   Item item;
 };
 
-// The piece that begins at tile t, n_tiles before the share's end; by a whole warp.
+// The piece that begins at unit u, `left` before the share's end; by a whole warp.
 template <int TK>
-__device__ __forceinline__ Piece piece_at(const Args& a, const Work& w, const Deal<kThreads>& d, int head_tiles,
-                                          int t, int n_tiles) {
+__device__ __forceinline__ Piece piece_at(const Args& a, const Work& w, const Deal<kThreads>& d, int head_units, int u,
+                                          int left) {
   Piece p;
-  p.head = t / head_tiles;
-  const int tt = t % head_tiles;
+  p.head = u / head_units;
   int at, n;
-  p.index = item_of<TK, kThreads>(a, w, d, tt, at, n);
-  p.item = w.items[p.index];
-  p.tiles = min(n - (tt - at), n_tiles);
-  p.left = n_tiles - p.tiles;
-  p.key0 = p.item.key0 + (tt - at) * TK;
-  p.continued = tt != at;
-  p.whole = p.tiles == n;
-  run_end(a, p.item, p.slot, p.end);
+  const int i = item_of<TK, kThreads>(a, w, d, u % head_units, at, n);
+  const Span s = span_of(w, u % head_units - at, n, left);
+  p.item = w.items[i];
+  p.units = s.units;
+  p.tiles = s.tiles;
+  p.key0 = p.item.key0 + s.tile0 * TK;
+  p.continued = s.tile0 > 0;
+  p.whole = s.whole;
+  if (p.tiles) run_end(a, p.item, p.slot, p.end);
   return p;
 }
 
@@ -195,11 +194,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   pdl_trigger();
   const Work& work = a.work[0];
-  const int head_tiles = deal<TK, kThreads>(a, work, dealt);
-  const int total = head_tiles * a.hk, size = share_size(work.workers, total, work.least);
+  const int head_units = deal<TK, kThreads>(a, work, dealt);
+  const int total = head_units * a.hk, size = share_size(work.workers, total, work.least);
   const int worker = warp * gridDim.x + blockIdx.x;  // few shares: spread over the SMs
-  const int t0 = worker * size, n_tiles = min(total - t0, size);
-  if (n_tiles <= 0) {
+  const int u0 = worker * size, units = min(total - u0, size);
+  if (units <= 0) {
     pdl_wait();
     return;
   }
@@ -207,8 +206,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   // The loads run ahead of the computation by the ring's stages, with a cursor of
   // their own (in, in_j); it holds the pages of up to 32 boxes of its piece, one a lane.
   const int box_rows = min(a.page, TK), boxes_of_tile = TK / box_rows;
-  Piece in = piece_at<TK>(a, work, dealt, head_tiles, t0, n_tiles), now = in;
-  int in_j = 0, page = 0, page_from = 0;  // boxes [page_from, page_from + 32) of the piece are in `page`
+  Piece in;
+  in.tiles = 0;
+  int in_j = 0, in_units = 0, loaded = 0;  // tiles loaded of the piece; units up to its end, tiles loaded of the share
+  int page = 0, page_from = 0;             // boxes [page_from, page_from + 32) of the piece are in `page`
   auto look_up = [&](int box) {
     page_from = box;
     const int key = in.key0 + (box + lane) * box_rows;
@@ -221,14 +222,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   };
-  look_up(0);
-  int loaded = 0;
   auto load_next = [&]() {
-    if (loaded == n_tiles) return;
-    if (in_j == in.tiles) {
-      in = piece_at<TK>(a, work, dealt, head_tiles, t0 + loaded, n_tiles - loaded);
+    while (in_j == in.tiles) {
+      if (in_units == units) return;
+      in = piece_at<TK>(a, work, dealt, head_units, u0 + in_units, units - in_units);
+      in_units += in.units;
       in_j = 0;
-      look_up(0);
+      if (in.tiles) look_up(0);
     }
     const int box0 = in_j * boxes_of_tile, k0 = in.key0 + in_j * TK;
     if (box0 + boxes_of_tile > page_from + 32) look_up(box0);
@@ -258,10 +258,18 @@ __global__ void __launch_bounds__(kThreads, 2)
   Acc<D> acc;
   uint32_t qf[D / 16][4];
   int lim[2];
-  int j = now.tiles;  // so that the first tile begins a piece
-  for (int i = 0; i < n_tiles; ++i) {
+  Piece now;
+  now.tiles = 0;
+  int j = 0, now_units = 0;
+  bool more = true;
+  for (int i = 0;; ++i) {
     if (j == now.tiles) {
-      if (i > 0) now = piece_at<TK>(a, work, dealt, head_tiles, t0 + i, n_tiles - i);
+      do {
+        if (!(more = now_units < units)) break;
+        now = piece_at<TK>(a, work, dealt, head_units, u0 + now_units, units - now_units);
+        now_units += now.units;
+      } while (now.tiles == 0);
+      if (!more) break;
       j = 0;
       acc.clear();
 #pragma unroll
@@ -352,11 +360,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
   for (int s = 0; s < 2; ++s) {
     if (item[s] < 0) continue;
     const Work& w = item[s] >= kBig ? a.work[1] : a.work[0];
-    const int i = item[s] & (kBig - 1), all = w.tile0[w.n], first = w.tile0[i], n = w.tile0[i + 1] - first;
+    const int i = item[s] & (kBig - 1), all = w.unit0[w.n], first = w.unit0[i], n = w.unit0[i + 1] - first;
     if (n == 0) continue;
-    const int size = share_size(w.workers, all * a.hk, w.least), t = head * all + first;
-    c0[s] = t / size;
-    count[s] = (t + n - 1) / size - c0[s] + 1;
+    const int size = share_size(w.workers, all * a.hk, w.least), u = head * all + first;
+    c0[s] = (u + w.over) / size;
+    count[s] = (u + n - 1) / size - c0[s] + 1;
   }
   const int parts = count[0] + count[1];
   if (parts == 1 && (item[0] < 0 || item[1] < 0)) return;  // its only piece wrote the output
@@ -567,7 +575,12 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
     w.workers = i ? sms : 2 * kWarps * sms;
     w.item_rows = i ? kBigRows : kSmallRows;
     w.continued = slots;
-    w.least = i ? 1 : 2;  // a share of one tile leaves more to join than it saves
+    // Swept from 0 to 4 on calls of 4 to 300 sequences: a worker's time for a piece
+    // without its tiles is that of about three tiles in both kernels (none counted: 5
+    // to 25 % slower where pieces are short). Shares of fewer than four units leave
+    // more to join than they save.
+    w.over = 3;
+    w.least = i ? 1 : 4;
     if (w.n == 0) continue;
     slots += int64_t(w.workers) * w.item_rows;
     firsts += w.n + 1;
@@ -575,8 +588,8 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   auto ws = torch::empty({slots * (d + 2) + firsts}, q.options().dtype(at::kFloat));
   a.part_o = ws.data_ptr<float>();
   a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * d);
-  a.work[0].tile0 = reinterpret_cast<int*>(a.part_ml + slots);
-  a.work[1].tile0 = a.work[0].tile0 + (a.work[0].n ? a.work[0].n + 1 : 0);
+  a.work[0].unit0 = reinterpret_cast<int*>(a.part_ml + slots);
+  a.work[1].unit0 = a.work[0].unit0 + (a.work[0].n ? a.work[0].n + 1 : 0);
   const int *si = shared_item.data_ptr<int>(), *oi = own_item.data_ptr<int>();
   if (type == at::kBFloat16 && d == 128) launch<__nv_bfloat16, 128>(k, v, a, si, oi);
   else if (type == at::kBFloat16) launch<__nv_bfloat16, 64>(k, v, a, si, oi);

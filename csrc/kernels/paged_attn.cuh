@@ -24,17 +24,19 @@ struct Item {
   int alone;   // its pairs have no other run of keys
 };
 
-// The items of one kernel. Their tiles are numbered one after another, head by
-// head, and every worker (a warp, or a CTA) takes an equal contiguous share of the
-// numbers.
+// The items of one kernel. Their units are numbered one after another, head by head,
+// and every worker (a warp, or a CTA) takes an equal contiguous share of the numbers.
+// An item with keys has `over` units for what a worker spends on any item (look-ups,
+// Q, write-out), then one for each tile of its keys.
 struct Work {
   const Item* items;
   int n;           // items of one head
   int workers;
-  int* tile0;      // n + 1: first tile of each item, of one head (written by CTA 0)
+  int over;
+  int* unit0;      // n + 1: first unit of each item, of one head (written by CTA 0)
   long continued;  // partial slots of the workers' pieces that continue an earlier worker's
   int item_rows;   // slots of each
-  int least;       // tiles of a share
+  int least;       // units of a share, at least
 };
 constexpr int kSmallRows = 16;
 constexpr int kBig = 1 << 30;  // marks an item of work[1] in the join's lists
@@ -76,12 +78,12 @@ __device__ __forceinline__ int length_of(const Args& a, int slot) {
 }
 
 template <int TK>
-__device__ __forceinline__ int tiles_of(const Args& a, const Item& it) {
+__device__ __forceinline__ int units_of(const Args& a, const Work& w, const Item& it) {
   const int keys = it.shared ? it.keys : length_of(a, it.first) - it.keys - it.key0;
-  return keys > 0 ? (keys + TK - 1) / TK : 0;
+  return keys > 0 ? w.over + (keys + TK - 1) / TK : 0;
 }
 
-// Tiles are dealt in shares of equal size (the last one may be shorter): worker c
+// Units are dealt in shares of equal size (the last one may be shorter): worker c
 // takes [c * size, (c + 1) * size) of `total`.
 __device__ __forceinline__ int share_size(int workers, int total, int least) {
   return max((total + workers - 1) / workers, least);
@@ -96,23 +98,23 @@ __device__ __forceinline__ long continued_slot(const Work& w, int worker, int pa
   return w.continued + long(worker) * w.item_rows + (pair & (w.item_rows - 1));
 }
 
-// The first tile of every item, in shared memory while there are few items; of more,
+// The first unit of every item, in shared memory while there are few items; of more,
 // only of each thread's run [t * per, (t + 1) * per).
 constexpr int kFirsts = 512;
 template <int THREADS>
 struct Deal {
-  int run[THREADS + 1];  // tiles before each thread's run; the last entry: tiles of one head
+  int run[THREADS + 1];  // units before each thread's run; the last entry: units of one head
   int first[kFirsts + 1];
 };
 
-// Numbers the items' tiles; CTA 0 leaves every item's first tile for the joining
-// kernel. All THREADS threads of the CTA take part. Returns the tiles of one head.
+// Numbers the items' units; CTA 0 leaves every item's first one for the joining
+// kernel. All THREADS threads of the CTA take part. Returns the units of one head.
 template <int TK, int THREADS>
 __device__ __forceinline__ int deal(const Args& a, const Work& w, Deal<THREADS>& d) {
   const int tid = threadIdx.x, per = (w.n + THREADS - 1) / THREADS;
   const int i0 = min(w.n, tid * per), i1 = min(w.n, i0 + per);
   int mine = 0;
-  for (int i = i0; i < i1; ++i) mine += tiles_of<TK>(a, w.items[i]);
+  for (int i = i0; i < i1; ++i) mine += units_of<TK>(a, w, w.items[i]);
   d.run[tid] = mine;
   __syncthreads();
   if (tid < 32) {
@@ -135,24 +137,24 @@ __device__ __forceinline__ int deal(const Args& a, const Work& w, Deal<THREADS>&
     int t = d.run[tid];
     for (int i = i0; i < i1; ++i) {
       if (w.n <= kFirsts) d.first[i] = t;
-      if (blockIdx.x == 0) w.tile0[i] = t;
-      t += per == 1 ? mine : tiles_of<TK>(a, w.items[i]);
+      if (blockIdx.x == 0) w.unit0[i] = t;
+      t += per == 1 ? mine : units_of<TK>(a, w, w.items[i]);
     }
     if (tid == 0) {
       if (w.n <= kFirsts) d.first[w.n] = d.run[THREADS];
-      if (blockIdx.x == 0) w.tile0[w.n] = d.run[THREADS];
+      if (blockIdx.x == 0) w.unit0[w.n] = d.run[THREADS];
     }
   }
   __syncthreads();
   return d.run[THREADS];
 }
 
-// The item that holds tile t of a head; `at` becomes its first tile, `n` its tiles.
+// The item that holds unit t of a head; `at` becomes its first unit, `n` its units.
 template <int TK, int THREADS>
 __device__ __forceinline__ int item_of(const Args& a, const Work& w, const Deal<THREADS>& d, int t, int& at, int& n) {
   const bool few = w.n <= kFirsts;
   const int* first = few ? d.first : d.run;
-  int lo = 0, hi = (few ? w.n : THREADS) - 1;  // the last whose first tile is not past t
+  int lo = 0, hi = (few ? w.n : THREADS) - 1;  // the last whose first unit is not past t
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
     if (first[mid] <= t) lo = mid;
@@ -164,12 +166,26 @@ __device__ __forceinline__ int item_of(const Args& a, const Work& w, const Deal<
     return lo;
   }
   int i = lo * ((w.n + THREADS - 1) / THREADS);
-  n = tiles_of<TK>(a, w.items[i]);
+  n = units_of<TK>(a, w, w.items[i]);
   while (at + n <= t) {
     at += n;
-    n = tiles_of<TK>(a, w.items[++i]);
+    n = units_of<TK>(a, w, w.items[++i]);
   }
   return i;
+}
+
+// A worker's piece of an item: the units [u0, u0 + units) of the item's n are its.
+struct Span {
+  int units, tile0, tiles;
+  bool whole;  // all tiles of the item
+};
+__device__ __forceinline__ Span span_of(const Work& w, int u0, int n, int left) {
+  Span s;
+  s.units = min(n - u0, left);
+  s.tile0 = max(0, u0 - w.over);
+  s.tiles = max(0, u0 + s.units - w.over) - s.tile0;
+  s.whole = s.tiles == n - w.over;
+  return s;
 }
 
 // The table row that an item's keys are read through, and the end of those that

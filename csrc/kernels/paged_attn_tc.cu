@@ -2,7 +2,7 @@
 // tokens behind one prefix): the same sums as paged_attn.cu on the 5th-generation
 // tensor cores.
 //
-// One CTA an SM takes an equal share of all (item, 128-key tile) numbers and walks
+// One CTA an SM takes an equal share of all items' units and walks
 // it piece by piece (a piece: the part of an item that lies in its share). An item
 // is up to 256 (row, query head) pairs: two tiles of 128, so that one tile's MMAs
 // run under the other's softmax. Tensor memory holds S0, S1 and O0, O1. Roles:
@@ -34,12 +34,12 @@ namespace {
 
 constexpr int kThreads = 576;
 constexpr int kSoftWarps = 8;  // of one tile
-constexpr int kPieces = 8;  // records; the producer is at most four pieces ahead of the slowest role
+constexpr int kPieces = 8;  // records; the producer is at most five pieces ahead of the slowest role
 constexpr float kRescale = 8.f;
 
 struct Piece {
   int row0, rows, head, shared;
-  int key0, tiles;   // first key and tiles of the piece
+  int key0, tiles;   // first key and tiles of the piece (none: it ends the share)
   int end;           // keys of the item's run that exist
   int continued;
   int final;         // nothing to join: the piece writes the output
@@ -118,35 +118,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 1) tmem_alloc(&tmem_slot, 512);
   pdl_trigger();
-  const int head_tiles = deal<BK, kThreads>(a, w, dealt);
+  const int head_units = deal<BK, kThreads>(a, w, dealt);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(tmem_slot);  // S0 @0, S1 @128, O0 @256, O1 @256 + D
-  const int total = head_tiles * a.hk, size = share_size(w.workers, total, w.least);
-  const int t_begin = blockIdx.x * size, n_tiles = uniform(min(total - t_begin, size));  // none: n_tiles <= 0
+  const int total = head_units * a.hk, size = share_size(w.workers, total, w.least);
+  const int u_begin = blockIdx.x * size, n_units = uniform(min(total - u_begin, size));  // none: n_units <= 0
 
   if (warp == 0) {
     const int box_rows = min(a.page, BK);
-    int it = 0;  // tiles loaded
+    int it = 0, units = 0, p = 0;  // tiles loaded, units up to the end of the piece found last, pieces
     bool ok = true;
-    for (int p = 0; it < n_tiles && ok; ++p) {
-      const int t = t_begin + it, tt = t % head_tiles;
-      int at, n;
-      const int i = item_of<BK, kThreads>(a, w, dealt, tt, at, n);
-      const Item item = w.items[i];
-      int slot, end;
-      run_end(a, item, slot, end);
-      const int tiles = min(n - (tt - at), n_tiles - it), key0 = item.key0 + (tt - at) * BK, head = t / head_tiles;
+    Piece pc;
+    int slot = 0;
+    // Finds the share's next piece with tiles and leaves its record; after the last
+    // one, a record without.
+    auto find = [&]() {
+      pc = Piece{};
+      while (pc.tiles == 0 && units < n_units) {
+        const int u = u_begin + units;
+        int at, n;
+        const int i = item_of<BK, kThreads>(a, w, dealt, u % head_units, at, n);
+        const Item item = w.items[i];
+        const Span s = span_of(w, u % head_units - at, n, n_units - units);
+        units += s.units;
+        if (s.tiles == 0) continue;
+        int end;
+        run_end(a, item, slot, end);
+        pc = Piece{item.row0, item.rows, u / head_units, item.shared, item.key0 + s.tile0 * BK, s.tiles, end,
+                   s.tile0 > 0, item.alone && s.whole};
+      }
       if (lane == 0) {
-        pieces[p % kPieces] = Piece{item.row0, item.rows, head, item.shared, key0, tiles, end, tt != at,
-                                   item.alone && tiles == n};
+        pieces[p % kPieces] = pc;
         mbar_arrive(&piece_full[p % kPieces]);
       }
+      ++p;
+    };
+    find();
+    while (pc.tiles && ok) {
+      const int key0 = pc.key0, tiles = pc.tiles, head = pc.head, end = pc.end, row_slot = slot;
       auto page_of = [&](int j) {  // of this lane's box of tile j of the piece
         const int key = key0 + j * BK + lane * box_rows;
         if (lane * box_rows >= BK || key >= end || j >= tiles) return 0;
-        int page = a.table[long(slot) * a.width + key / a.page];
+        int page = a.table[long(row_slot) * a.width + key / a.page];
         if (page < 0 || page >= a.pages) {
           atomicCAS(a.err, 0, kErrBounds);
           page = 0;
@@ -176,6 +191,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < D / 64; ++c)
             tma_load_3d(sV + b * S::kTile + c * S::kSub + lane * box_rows * 128, &tm_v, &v_full[b], c * 64, row, page);
         page = next;
+        // The next piece is found while this one's tiles are at work.
+        if (j == min(1, tiles - 1)) find();
       }
       ok = __all_sync(0xffffffffu, ok);
     }
@@ -219,9 +236,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (leader) umma_commit(bar);
       __syncwarp();
     };
-    for (int p = 0; it < n_tiles && ok; ++p) {
+    for (int p = 0; ok; ++p) {
       if (!(ok = wait(&piece_full[p % kPieces], (p / kPieces) & 1, kErrTimeoutMma, a.err))) break;
       const int rows = uniform(pieces[p % kPieces].rows), tiles = uniform(pieces[p % kPieces].tiles);
+      if (tiles == 0) break;
       const int keys = uniform(pieces[p % kPieces].end - pieces[p % kPieces].key0);
       const bool two = rows > 128;
       if (!(ok = wait(&q_full, p & 1, kErrTimeoutMma, a.err))) break;
@@ -279,9 +297,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       other = slot[half ^ 1][r];
       return done;
     };
-    for (int p = 0; it < n_tiles && ok; ++p) {
+    for (int p = 0; ok; ++p) {
       if (!wait(&piece_full[p % kPieces], (p / kPieces) & 1, kErrTimeoutEpilogue, a.err)) break;
       const Piece pc = pieces[p % kPieces];
+      if (pc.tiles == 0) break;
       const int pair = pc.row0 + t * 128 + r;
       const bool active = pc.rows > t * 128, mine = t * 128 + r < pc.rows;
       int lim = INT_MAX / 2;  // rows past the item's: computed on zeros, never written
@@ -309,7 +328,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) {
           const int c = c0 + i;
-          *reinterpret_cast<uint4*>(sQ + t * S::kTile + (c / 8) * S::kSub + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+          uint8_t* sub = sQ + t * S::kTile + (c / 8) * S::kSub;
+          *reinterpret_cast<uint4*>(sub + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
         }
         fence_proxy_async();
       }

@@ -74,9 +74,19 @@ def copy_pages(k, v, src, dst) -> None:
 
 
 # (row, query head) pairs of an item, as in csrc/kernels/paged_attn.cuh: up to
-# SMALL_ROWS on mma.sync, up to BIG_ROWS (two tiles of 128) on tcgen05.
-SMALL_ROWS, TILE_ROWS, BIG_ROWS, BIG = 16, 128, 256, 1 << 30
-APART, BIG_FROM = 1.25, 64
+# SMALL_ROWS on mma.sync, up to BIG_ROWS (two tiles of 128) on tcgen05. Runs of more
+# than BIG_FROM pairs go to tcgen05: 64 rows of one prefix of 1984 tokens take 30.6 us
+# as four items on mma.sync and 40.7 us there, 128 rows of 8192 tokens 87.7 and 65.2 us.
+SMALL_ROWS, BIG_ROWS, BIG_FROM, BIG = 16, 256, 64, 1 << 30
+
+
+def _cost(pairs, keys, over: int):
+    """Time of a run of ``keys`` keys for ``pairs`` pairs, in tiles of the tcgen05
+    kernel (2.3 us of an SM); a tile of a warp on mma.sync takes 0.036 of one, and
+    an item as long as ``over`` tiles before its first."""
+    big = -(-pairs // BIG_ROWS) * (over + -(-keys // 128))
+    small = -(-pairs // SMALL_ROWS) * (over + -(-keys // 32)) * 0.036
+    return np.where(pairs > BIG_FROM, big, small)
 
 
 class PrefixPlan:
@@ -128,12 +138,14 @@ class PrefixPlan:
         at = 0
         own_from = np.zeros(n_seq, np.int64)
         for n, shared in groups:
-            # Rows of several sequences fill the tiles of the shared keys better than
-            # each sequence's own would; where they barely do (prompts of many tokens),
-            # one run over all keys saves the joining of two.
+            # The shared keys as a run of their own, for the rows of all: its tiles are
+            # fuller, but it is an item more and every pair has two runs to join (0.018
+            # of a tile's time for 100 values). Prompts of many tokens fill their tiles
+            # alone, and short prefixes are soon read again.
             pairs = t[at:at + n] * share
-            apart, together = (-(-pairs // TILE_ROWS)).sum(), -(-pairs.sum() // TILE_ROWS)
-            if n > 1 and shared > 0 and apart > APART * together:
+            apart = _cost(pairs, shared, 0).sum()
+            together = _cost(pairs.sum(), shared, 3) + pairs.sum() * head_dim * 1.8e-4
+            if n > 1 and shared > 0 and apart > together:
                 add(1, at, n, start[at], start[at + n], 0, shared)
                 own_from[at:at + n] = shared
             at += n

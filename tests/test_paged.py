@@ -596,17 +596,28 @@ def test_plan_refusals_cpu(kw):
         paged.PrefixPlan(**{**args, **kw})
 
 
-def test_plan_items_cpu():
-    """Every (row, head) pair is in one item of its own keys, and in one of the shared keys where its group shares."""
+@pytest.mark.parametrize("groups,q_lens,split", [
+    ([(1, 64), (3, 32), (2, 0)], [3, 40, 1, 0, 2, 5], [0, 0, 0, 0, 0, 0]),        # too short a prefix to be worth a run
+    ([(1, 6400), (3, 3200), (2, 0)], [3, 40, 1, 0, 2, 5], [0, 1, 1, 1, 0, 0]),
+    ([(2, 3200), (9, 3200)], [300, 200] + [1] * 9, [0, 0] + [1] * 9),             # long prompts fill their tiles alone
+])
+def test_plan_items_cpu(groups, q_lens, split):
+    """Every (row, head) pair is in one item of its own keys, and in one of the shared keys where its group is
+    split; own keys begin where the shared run ends, or at 0."""
     from rs_nanogpt_b200.ops import paged
-    plan = paged.PrefixPlan([(1, 64), (3, 32), (2, 0)], [3, 40, 1, 0, 2, 5], n_head=6, n_kv_head=2, head_dim=64,
-                            page=32, table_width=8, device="cpu")
-    seen = {0: [0] * (51 * 3), 1: [0] * (51 * 3)}
+    plan = paged.PrefixPlan(groups, q_lens, n_head=6, n_kv_head=2, head_dim=64, page=32, table_width=256, device="cpu")
+    shared_of = [s for n, s in groups for _ in range(n)]
+    seq = [i for i, t in enumerate(q_lens) for _ in range(3 * t)]
+    seen = {0: [0] * len(seq), 1: [0] * len(seq)}
     for list_, most, mark in ((plan.items, 16, 0), (plan.big_items, 256, paged.BIG)):
-        for i, (shared, first, count, row0, rows, *_) in enumerate(list_.tolist()):
+        for i, (shared, first, count, row0, rows, key0, keys, alone) in enumerate(list_.tolist()):
             assert 0 < rows <= most
             for p in range(row0, row0 + rows):
                 seen[shared][p] += 1
                 assert (plan.shared_item if shared else plan.own_item)[p] == i + mark
-    assert seen[0] == [1] * 153
-    assert seen[1] == [0] * 9 + [1] * (41 * 3) + [0] * 21
+                if shared:
+                    assert (key0, keys) == (0, shared_of[seq[p]])
+                else:
+                    assert key0 == split[seq[p]] * shared_of[seq[p]] and alone == (key0 == 0)
+    assert seen[0] == [1] * len(seq)
+    assert seen[1] == [split[i] for i in seq]
