@@ -598,7 +598,7 @@ def test_plan_refusals_cpu(kw):
 
 @pytest.mark.parametrize("groups,q_lens,split", [
     ([(1, 64), (3, 32), (2, 0)], [3, 40, 1, 0, 2, 5], [0, 0, 0, 0, 0, 0]),        # too short a prefix to be worth a run
-    ([(1, 6400), (3, 3200), (2, 0)], [3, 40, 1, 0, 2, 5], [0, 1, 1, 1, 0, 0]),
+    ([(1, 6400), (30, 3200), (2, 0)], [3] + [5] * 29 + [0, 2, 5], [0] + [1] * 30 + [0, 0]),
     ([(2, 3200), (9, 3200)], [300, 200] + [1] * 9, [0, 0] + [1] * 9),             # long prompts fill their tiles alone
 ])
 def test_plan_items_cpu(groups, q_lens, split):
