@@ -3,6 +3,7 @@
 * ``generate``   KV-cache generation: p50 time to first token and decode tokens/s
 * ``attention``  causal flash attention fwd+bwd: error and TFLOP/s vs references
 * ``gemm``       tcgen05 GEMM at the d20 shapes vs cuBLAS
+* ``samples``    completions of one prompt: shared prefix (paged cache) vs repeated prompt
 * ``ddp_sweep``  fused reduce-scatter + AdamW + all-gather vs NCCL, per bucket size
 
 All timings are CUDA events on the launching stream after warm-up; multi-GPU
