@@ -180,6 +180,19 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   const int heads = a.hq + 2 * a.hk;
   if (group >= a.rows * heads) return;  // whole groups leave; the shuffles name only their own lanes
   const int row = group / heads, h = group % heads;
+  const bool is_q = h < a.hq, is_v = h >= a.hq + a.hk;
+  const Heads& t = is_q ? a.q : (is_v ? a.v : a.k);
+  const int i = is_q ? h : (is_v ? h - a.hq - a.hk : h - a.hq);
+  // The values are on their way while the row's place is looked up.
+  const T* src = static_cast<const T*>(t.src) + row * t.src_row + i * t.src_head;
+  Vec<T, V> va[NI], vb[NI];
+  int oa[NI], ob[NI];
+#pragma unroll
+  for (int n = 0; n < NI; ++n) {
+    item_offsets<V>(lane + n * L, a.half, a.interleaved, oa[n], ob[n]);
+    va[n] = *reinterpret_cast<const Vec<T, V>*>(src + oa[n]);
+    vb[n] = *reinterpret_cast<const Vec<T, V>*>(src + ob[n]);
+  }
   const int slot = a.row_slot[row];
   if (slot < 0 || slot >= a.slots) {
     if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
@@ -187,14 +200,10 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   }
   const int p = a.lens[slot] - 1 - a.row_back[row];
   if (p < 0) return;  // a slot that holds fewer tokens than its rows: nothing to write
-  const bool is_q = h < a.hq, is_v = h >= a.hq + a.hk;
   if (p >= a.positions || p >= a.width * a.page) {
     if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
     return;
   }
-  const Heads& t = is_q ? a.q : (is_v ? a.v : a.k);
-  const int i = is_q ? h : (is_v ? h - a.hq - a.hk : h - a.hq);
-  const T* src = static_cast<const T*>(t.src) + row * t.src_row + i * t.src_head;
   T* dst;
   if (is_q) {
     dst = static_cast<T*>(t.dst) + row * t.dst_row + i * t.dst_head;
@@ -205,14 +214,6 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
       return;
     }
     dst = static_cast<T*>(t.dst) + page * t.dst_row + i * t.dst_head + long(p % a.page) * D;
-  }
-  Vec<T, V> va[NI], vb[NI];
-  int oa[NI], ob[NI];
-#pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    item_offsets<V>(lane + n * L, a.half, a.interleaved, oa[n], ob[n]);
-    va[n] = *reinterpret_cast<const Vec<T, V>*>(src + oa[n]);
-    vb[n] = *reinterpret_cast<const Vec<T, V>*>(src + ob[n]);
   }
   if (!is_v) {
     float x[NI][2 * V], sq = 0.f;

@@ -32,6 +32,7 @@ class _Counted:
             _count[0] += n(*args, **kwargs) if callable(n) else n
             return fn(*args, **kwargs)
 
+        self.__dict__[name] = call  # looked up and wrapped once
         return call
 
 
