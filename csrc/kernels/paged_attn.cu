@@ -21,6 +21,11 @@
 // its own by TMA and keeps the running maximum and sum in registers. No warp waits
 // for another, so the look-ups, first loads and write-outs of one run under the
 // loads of the others on its SM. Items of more pairs: paged_attn_tc.cu.
+//
+// Measured (one B200): the own keys of 256 requests, 268 MB, in 58 us (4.6 TB/s); 64
+// samples of one prompt of 1984 tokens, ten heads of 128, in 23 us with the join,
+// where look-ups and partials, not bytes (7 us), are the time. CTAs whose four warps
+// shared tiles and met at barriers took 27 us for that call's first kernel, these 21.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>

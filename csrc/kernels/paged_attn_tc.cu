@@ -18,6 +18,11 @@
 //               stale maximum scales P and O alike.
 // Keys past the end of an item's run are hidden by the mask; their values are
 // cleared in shared memory first, since 0 * NaN is not 0.
+//
+// Measured (one B200): 1024 rows against 32768 keys on 4 kv heads of 128 (69 GFLOP) in
+// 81 us, 849 TFLOP/s; a tile of 256 rows and 128 keys takes about 3600 cycles, of which
+// the MMAs need 2048 and the exponentials as many: what is left is the way between the
+// two (scores ready, maximum, P stored, MMA issued), which two tiles do not quite hide.
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
 

@@ -6,8 +6,8 @@
 * ``samples``    completions of one prompt: shared prefix (paged cache) vs repeated prompt
 * ``ddp_sweep``  fused reduce-scatter + AdamW + all-gather vs NCCL, per bucket size
 
-All timings are CUDA events on the launching stream after warm-up; multi-GPU
-numbers are the max over ranks.
+All timings are CUDA events on the launching stream after warm-up (``samples``:
+wall clock of whole calls); multi-GPU numbers are the max over ranks.
 """
 
 
