@@ -295,7 +295,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     const int st = i % kStages, k0 = now.key0 + j * TK, valid = min(TK, max(0, now.end - k0));
-    if (!wait(&full[st], (i / kStages) & 1, kErrTimeoutMma, a.err)) return;
+    if (!wait(&full[st], (i / kStages) & 1, kErrTimeoutMma, a.err)) {
+      // The other stage's copies may still be on their way into this CTA's memory.
+      if (loaded > i + 1) wait(&full[(i + 1) % kStages], ((i + 1) / kStages) & 1, kErrTimeoutMma, a.err);
+      return;
+    }
     uint8_t* tile = ring + st * 2 * R::kTile;
     if (valid < TK) {
       // Rows past the last key hold what the page or an earlier tile held, which
@@ -539,7 +543,9 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   TORCH_CHECK(shared_item.numel() == rows * share, "paged_attention: the plan is for ",
               num(rows ? shared_item.numel() / rows : 0), " query heads a kv head, q has ", num(share));
   TORCH_CHECK(scale > 0, "paged_attention: scale must be positive");
-  TORCH_CHECK(rows * hq <= (int64_t(1) << 30) && table.size(1) * page <= INT32_MAX, "paged_attention: sizes");
+  TORCH_CHECK(rows * hq <= (int64_t(1) << 28) && table.size(1) * page <= INT32_MAX &&
+                  (items.size(0) + big_items.size(0)) * hk * (4 + table.size(1) * page / 32) <= INT32_MAX,
+              "paged_attention: more rows or tiles than 32-bit numbers count");
   if (lse.has_value()) {
     TORCH_CHECK(lse->device() == q.device() && lse->scalar_type() == at::kFloat && lse->is_contiguous() &&
                     lse->dim() == 2 && lse->size(0) == rows && lse->size(1) == hq,

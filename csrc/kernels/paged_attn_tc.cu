@@ -201,6 +201,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ok = __all_sync(0xffffffffu, ok);
     }
+    // After a wait that ran out: copies may still be on their way into this CTA's memory.
+    for (int x = max(0, it - 2); !ok && x <= it; ++x) {
+      wait(&k_full[x & 1], (x >> 1) & 1, kErrTimeoutProducer, a.err);
+      wait(&v_full[x & 1], (x >> 1) & 1, kErrTimeoutProducer, a.err);
+    }
   } else if (warp == 1) {
     // The whole warp walks the loop and one lane issues: descriptors and phases stay
     // in uniform registers, which the MMA instruction reads. With the loop itself

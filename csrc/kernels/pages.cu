@@ -350,11 +350,12 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs
   const int n = a.count ? min(*a.count, a.n) : a.n;
   const long units = long(n) * a.layers * 2 * a.heads;
   for (long u = long(blockIdx.x) * (kCopyThreads / 32) + threadIdx.x / 32; u < units; u += warps) {
+    // All pairs of one layer's k or v, then the next: what is written at a time lies
+    // in a few slices of the pool instead of all over it.
     const int head = int(u % a.heads);
-    long w = u / a.heads;
-    const bool is_v = w & 1;
-    w >>= 1;
-    const int layer = int(w % a.layers), pair = int(w / a.layers);
+    const long w = u / a.heads;
+    const int pair = int(w % n), slice = int(w / n), layer = slice / 2;
+    const bool is_v = slice & 1;
     const int from = a.src[pair], to = a.dst[pair];
     if (from < 0) continue;
     if (from >= a.pages || to < 0 || to >= a.pages) {
