@@ -255,17 +255,37 @@ __global__ void __launch_bounds__(kThreads, 2)
     ++in_j;
     ++loaded;
   };
-#pragma unroll
-  for (int i = 0; i < kStages; ++i) load_next();
-
   const int g = lane >> 2, t4 = lane & 3;
   const T* Q = static_cast<const T*>(a.q);
   Acc<D> acc;
   uint32_t qf[D / 16][4];
   int lim[2];
-  Piece now;
-  now.tiles = 0;
-  int j = 0, now_units = 0;
+  auto begin = [&](const Piece& p) {
+    acc.clear();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rr = g + 8 * e;
+      lim[e] = INT_MAX / 2;  // rows past the item's: computed on zeros, never written
+      const T* src = nullptr;
+      if (rr < p.item.rows) {
+        const int row = (p.item.row0 + rr) / a.share, h = (p.item.row0 + rr) % a.share;
+        lim[e] = length_of(a, a.row_slot[row]) - a.row_back[row];
+        src = Q + row * a.q_row + (p.head * a.share + h) * a.q_head;
+      }
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][e] = src ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + t4 * 2) : 0u;
+        qf[kk][e + 2] = src ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + t4 * 2) : 0u;
+      }
+    }
+  };
+  // The first piece is known from its first load; its Q comes while the tiles do.
+  load_next();
+  Piece now = in;
+  int j = 0, now_units = in_units;
+  if (now.tiles) begin(now);
+#pragma unroll
+  for (int i = 1; i < kStages; ++i) load_next();
   bool more = true;
   for (int i = 0;; ++i) {
     if (j == now.tiles) {
@@ -276,23 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       } while (now.tiles == 0);
       if (!more) break;
       j = 0;
-      acc.clear();
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int rr = g + 8 * e;
-        lim[e] = INT_MAX / 2;  // rows past the item's: computed on zeros, never written
-        const T* src = nullptr;
-        if (rr < now.item.rows) {
-          const int row = (now.item.row0 + rr) / a.share, h = (now.item.row0 + rr) % a.share;
-          lim[e] = length_of(a, a.row_slot[row]) - a.row_back[row];
-          src = Q + row * a.q_row + (now.head * a.share + h) * a.q_head;
-        }
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][e] = src ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + t4 * 2) : 0u;
-          qf[kk][e + 2] = src ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + t4 * 2) : 0u;
-        }
-      }
+      begin(now);
     }
     const int st = i % kStages, k0 = now.key0 + j * TK, valid = min(TK, max(0, now.end - k0));
     if (!wait(&full[st], (i / kStages) & 1, kErrTimeoutMma, a.err)) {
