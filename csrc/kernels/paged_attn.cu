@@ -6,14 +6,14 @@
 // over the keys j < limit(r) = lens[slot(r)] - back(r) of the row's sequence: the
 // row sees every token up to its own. A row without keys gives 0 (LSE -inf).
 //
-// The work of one kv head is a list of items, made once for a plan: an item is up
-// to 64 (row, query head) pairs against a run of keys, either the shared pages of
-// a group (rows of all its sequences) or the rest of one sequence. Tiles of 64
-// keys of all items are numbered one after another and the CTAs take equal
-// contiguous shares, whatever the lengths are; they are read on the device, so a
-// captured graph follows them. Where a share ends inside an item, both CTAs leave
-// a partial (max, sum, unnormalised output, fp32); a second kernel joins a row's
-// partials from the shared keys and from its own.
+// The work of one kv head is a list of items, made once for a plan: an item is some
+// (row, query head) pairs against a run of keys, either the shared pages of a group
+// (rows of all its sequences) or the rest of one sequence. The items' tiles of keys
+// are numbered one after another and the workers take equal contiguous shares,
+// whatever the lengths are; they are read on the device, so a captured graph follows
+// them. Where a share ends inside an item, both workers leave a partial (max, sum,
+// unnormalised output, fp32); a last kernel joins a row's partials from the shared
+// keys and from its own.
 //
 // Here: items of up to 16 pairs (single tokens) on mma.sync, which is far from the
 // bound for so few rows; what counts is to keep loads in flight. A warp is a worker
