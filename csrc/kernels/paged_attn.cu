@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!wait(&full[st], (i / kStages) & 1, kErrTimeoutMma, a.err)) {
       // The other stage's copies may still be on their way into this CTA's memory.
       if (loaded > i + 1) wait(&full[(i + 1) % kStages], ((i + 1) / kStages) & 1, kErrTimeoutMma, a.err);
-      return;
+      break;
     }
     uint8_t* tile = ring + st * 2 * R::kTile;
     if (valid < TK) {

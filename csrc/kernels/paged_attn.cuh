@@ -59,12 +59,15 @@ struct Args {
 };
 
 // mbar_wait that polls for a while before it first reads the timer, which would
-// otherwise stand in the path of every wait that has to wait at all.
+// otherwise stand in the path of every wait that has to wait at all. By a whole warp,
+// with one answer for all its lanes: a warp that gives up leaves its role as a whole,
+// so that none of its lanes stands at a barrier, shuffle or tensor-memory access that
+// the others no longer reach.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int code, int* err) {
 #pragma unroll 1
   for (int i = 0; i < 64; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, code, err);
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code, err));
 }
 
 // 1 / sum; 0 for a row without keys, NaN where the sum is.

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int boxes = k0 < end ? (min(end - k0, BK) + box_rows - 1) / box_rows : 0;
         const int row = head * a.page + (k0 + lane * box_rows) % a.page;
         ok = wait(&k_empty[b], ((it >> 1) & 1) ^ 1, kErrTimeoutProducer, a.err);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&k_full[b], boxes * box_rows * D * 2);
         __syncwarp();
         if (lane < boxes)
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < D / 64; ++c)
             tma_load_3d(sK + b * S::kTile + c * S::kSub + lane * box_rows * 128, &tm_k, &k_full[b], c * 64, row, page);
         ok = wait(&v_empty[b], ((it >> 1) & 1) ^ 1, kErrTimeoutProducer, a.err);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&v_full[b], boxes * box_rows * D * 2);
         __syncwarp();
         if (lane < boxes)
@@ -199,7 +199,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The next piece is found while this one's tiles are at work.
         if (j == min(1, tiles - 1)) find();
       }
-      ok = __all_sync(0xffffffffu, ok);
     }
     // After a wait that ran out: copies may still be on their way into this CTA's memory.
     for (int x = max(0, it - 2); !ok && x <= it; ++x) {
