@@ -122,6 +122,8 @@ class PagedDecoder:
         lens = [len(t) for t in tokens]
         if not lens or min(lens) == 0 or len(slots) != len(tokens) or len(set(slots)) != len(slots):
             raise ValueError("feed: one slot of its own and at least one token for each sequence")
+        if min(slots) < 0 or max(slots) >= self.cache.lens.shape[0]:
+            raise ValueError(f"feed: slots must be below {self.cache.lens.shape[0]}, got {list(slots)}")
         dev = self.store.device
         add = torch.zeros_like(self.cache.lens)
         add[torch.tensor(list(slots), device=dev)] = torch.tensor(lens, dtype=torch.int32, device=dev)

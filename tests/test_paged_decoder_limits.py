@@ -1,0 +1,56 @@
+"""The decoder over the paged cache: what it refuses, what a refusal leaves behind, and its numbers with
+output projections that let the attention through."""
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+checked = pytest.mark.usefixtures("kernel_ok")
+
+
+def _store(seq=512, vocab=1000, depth=2):
+    """Random weights; the output projections, too, are drawn, so that the logits depend on the attention."""
+    from rs_nanogpt_b200.config import d_model
+    from rs_nanogpt_b200.models.params import ParamStore, init_params
+    cfg = d_model(depth, vocab_size=vocab, sequence_len=seq)
+    store = ParamStore(cfg, "cuda")
+    init_params(store, seed=5, mode="bench")
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for name in store.names():
+        if name.endswith("c_proj.weight"):
+            store.param(name).normal_(0.0, 0.05, generator=g)
+    store.refresh_work()
+    return cfg, store
+
+
+def _tokens(cfg, n, seed=0):
+    return torch.randint(0, cfg.vocab_size, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def _state(dec):
+    c = dec.cache
+    return [x.clone() for x in (c.table, c.lens, c.refs, c.k, c.v)]
+
+
+def _unchanged(dec, was):
+    return all(torch.equal(a, b) for a, b in zip(_state(dec), was))
+
+
+def _close(got, ref):
+    # bf16 activations through two blocks against fp32: the tolerance of the contiguous cache's test.
+    assert (got.float() - ref).abs().max().item() <= 5e-2 * max(1.0, ref.abs().max().item())
+
+
+@gpu
+@pytest.mark.usefixtures("kernel_ok")
+@pytest.mark.parametrize("slots", [[0, 8], [8], [0, -1], [-1], [1 << 40, 0]])
+def test_slots_outside_the_cache_are_refused(slots):
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    cfg, store = _store()
+    dec = PagedDecoder(store, pages=20, max_seqs=8, max_len=200, page=32)
+    dec.feed([_tokens(cfg, 40)], [7])
+    was = _state(dec)
+    with pytest.raises(ValueError):
+        dec.feed([[1]] * len(slots), slots)
+    assert _unchanged(dec, was)
