@@ -43,6 +43,33 @@ def _close(got, ref):
 
 
 @gpu
+@checked
+def test_logits_that_depend_on_the_attention():
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    from rs_nanogpt_b200.models.reference import ReferenceGpt
+    cfg, store = _store()
+    ref = ReferenceGpt(store, torch.float32)
+    dec = PagedDecoder(store, pages=40, max_seqs=8, max_len=400, page=32)
+
+    def expect(seqs):
+        return torch.stack([ref.forward(torch.tensor([s], device="cuda"))[0, -1] for s in seqs])
+
+    system = [_tokens(cfg, 130), _tokens(cfg, 70, 1)]
+    _close(dec.feed(system, [0, 4]), expect(system))
+    # They do depend on it: without the first half of a prompt they are others.
+    a, b = expect([system[0]]), expect([system[0][65:]])
+    assert (a - b).abs().max() > 0.3 * max(1.0, a.abs().max().item())
+    dec.cache.fork([0, 0, 4], [1, 2, 5])
+    slots, groups = [0, 1, 2, 4, 5], [(3, 128), (2, 64)]
+    seqs = [system[0] for _ in range(3)] + [system[1] for _ in range(2)]
+    for i, lens in enumerate(([5, 40, 1, 33, 7], [1] * 5, [2, 3, 4, 5, 6], [1] * 5)):
+        new = [_tokens(cfg, n, 10 * i + j + 2) for j, n in enumerate(lens)]
+        seqs = [s + t for s, t in zip(seqs, new)]
+        _close(dec.feed(new, slots, groups), expect(seqs))
+    dec.cache.check()
+
+
+@gpu
 @pytest.mark.usefixtures("kernel_ok")
 @pytest.mark.parametrize("slots", [[0, 8], [8], [0, -1], [-1], [1 << 40, 0]])
 def test_slots_outside_the_cache_are_refused(slots):
