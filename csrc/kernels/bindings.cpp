@@ -62,14 +62,16 @@ void rotate(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor pos, 
 void paged_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, torch::Tensor v_pages,
                   torch::Tensor table, torch::Tensor lens, torch::Tensor row_slot, torch::Tensor row_back,
                   c10::optional<torch::Tensor> cos_t, c10::optional<torch::Tensor> sin_t, bool interleaved, double eps,
-                  bool norm, torch::Tensor q_out);
+                  bool norm, torch::Tensor q_out, c10::optional<torch::Tensor> room);
 void pages_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
                 torch::Tensor parents, torch::Tensor children, torch::Tensor table_out, torch::Tensor lens_out,
                 torch::Tensor refs_out);
 void pages_grow(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor add, int64_t page,
-                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out);
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out,
+                c10::optional<torch::Tensor> room);
 void pages_free(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor seqs,
-                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out);
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out,
+                c10::optional<torch::Tensor> room);
 void pages_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,
                    torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out);
 void pages_copy(torch::Tensor k, torch::Tensor v, torch::Tensor src, torch::Tensor dst);

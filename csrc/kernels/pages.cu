@@ -7,6 +7,8 @@
 //   table   (slots, width) int32: a sequence's pages in order, -1 past the last
 //   lens    (slots) int32: tokens of a sequence (0: the slot is empty)
 //   refs    (pages) int32: table entries that name the page (0: the page is free)
+//   room    (slots) int32, optional: tokens that grow granted and that are not written
+//           yet, so that the append can tell them from those the cache holds
 //
 // Full pages are shared between forks and never written again; a partly filled
 // page belongs to one sequence. New pages are the lowest free ones, handed out in
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(kMetaThreads)
 // ws list: free pages (pages).
 template <int C>
 __global__ void __launch_bounds__(kMetaThreads)
-    grow_meta_kernel(const PageState s, const int* __restrict__ add, int* ws) {
+    grow_meta_kernel(const PageState s, const int* __restrict__ add, int* room, int* ws) {
   __shared__ int sm[32];
   using team = Team<C>;
   const int gid = team::gid();
@@ -252,7 +254,10 @@ __global__ void __launch_bounds__(kMetaThreads)
         s.table[long(i) * s.width + have + e] = q;
         s.refs[q] = 1;
       }
-      if (add[i]) s.lens[i] = len + add[i];
+      if (add[i]) {
+        s.lens[i] = len + add[i];
+        if (room) room[i] += add[i];
+      }
     }
     rank += max(0, m);
   }
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kMetaThreads)
 
 template <int C>
 __global__ void __launch_bounds__(kMetaThreads)
-    free_meta_kernel(const PageState s, const int* __restrict__ seqs, int n) {
+    free_meta_kernel(const PageState s, const int* __restrict__ seqs, int n, int* room) {
   using team = Team<C>;
   const int gid = team::gid();
   copy_state<C>(s);
@@ -273,6 +278,7 @@ __global__ void __launch_bounds__(kMetaThreads)
       if (lane == 0) report(s.err, kErrBounds);
       continue;
     }
+    if (room && lane == 0) room[slot] = 0;
     // A slot that the list names twice is freed once.
     const int had = __shfl_sync(0xffffffffu, lane == 0 ? atomicExch(s.lens + slot, 0) : 0, 0);
     if (had <= 0) continue;
@@ -407,6 +413,13 @@ PageState state_of(const torch::Tensor& table, const torch::Tensor& lens, const 
                    int(refs.size(0)), int(page), error_word()};
 }
 
+int* room_of(const c10::optional<torch::Tensor>& room, const torch::Tensor& lens, const char* op) {
+  if (!room.has_value()) return nullptr;
+  check_int_vec(*room, op, lens);
+  TORCH_CHECK(room->sizes() == lens.sizes(), op, ": room must have one entry for each slot");
+  return room->data_ptr<int>();
+}
+
 CopyArgs pools_of(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& like, const char* op) {
   for (const auto* t : {&k, &v}) {
     TORCH_CHECK(t->is_cuda() && t->device() == like.device(), op, ": pages must be on ", place(like));
@@ -496,24 +509,26 @@ void pages_fork(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Te
 }
 
 void pages_grow(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor add, int64_t page,
-                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out) {
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out,
+                c10::optional<torch::Tensor> room) {
   const PageState s = state_of(table, lens, refs, table_out, lens_out, refs_out, page, "grow_pages");
   check_int_vec(add, "grow_pages: add", table);
   TORCH_CHECK(add.sizes() == lens.sizes(), "grow_pages: add must have one entry for each slot");
   const at::cuda::CUDAGuard guard(table.device());
   auto ws = workspace(table, s.pages);
   launch_team(s, "grow_pages", grow_meta_kernel<1>, grow_meta_kernel<kMetaCtas>, add.data_ptr<int>(),
-              ws.data_ptr<int>());
+              room_of(room, lens, "grow_pages"), ws.data_ptr<int>());
 }
 
 void pages_free(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, torch::Tensor seqs,
-                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out) {
+                torch::Tensor table_out, torch::Tensor lens_out, torch::Tensor refs_out,
+                c10::optional<torch::Tensor> room) {
   const PageState s = state_of(table, lens, refs, table_out, lens_out, refs_out, 1, "free_pages");
   check_int_vec(seqs, "free_pages: seqs", table);
   TORCH_CHECK(seqs.dim() == 1, "free_pages: seqs must be a vector");
   const at::cuda::CUDAGuard guard(table.device());
   launch_team(s, "free_pages", free_meta_kernel<1>, free_meta_kernel<kMetaCtas>, seqs.data_ptr<int>(),
-              int(seqs.size(0)));
+              int(seqs.size(0)), room_of(room, lens, "free_pages"));
 }
 
 void pages_compact(torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens, torch::Tensor refs,

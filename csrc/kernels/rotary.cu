@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotate_kernel(const RotateArgs
 struct AppendArgs {
   Heads q, k, v;  // k.dst, v.dst: the layer's pages; *_row: elements a page, *_head: elements a head of a page
   const int *table, *lens, *row_slot, *row_back;
+  const int* room;             // tokens of a slot that were granted and not yet written; null: nothing is known
   const float *cos_t, *sin_t;  // null: no turn
   int rows, hq, hk, half, positions, page, width, pages, slots;
   float eps;
@@ -200,8 +201,12 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
     return;
   }
-  const int p = a.lens[slot] - 1 - a.row_back[row];
+  const int back = a.row_back[row], p = a.lens[slot] - 1 - back;
   if (p < 0) return;  // a slot that holds fewer tokens than its rows: nothing to write
+  if (a.room && back >= a.room[slot]) {  // the place of a token that the cache already holds
+    if (lane == 0) atomicCAS(a.err, 0, kErrNoPages);
+    return;
+  }
   if (p >= a.positions || p >= a.width * a.page) {
     if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
     return;
@@ -414,7 +419,7 @@ void rotate(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor pos, 
 void paged_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, torch::Tensor v_pages,
                   torch::Tensor table, torch::Tensor lens, torch::Tensor row_slot, torch::Tensor row_back,
                   c10::optional<torch::Tensor> cos_t, c10::optional<torch::Tensor> sin_t, bool interleaved, double eps,
-                  bool norm, torch::Tensor q_out) {
+                  bool norm, torch::Tensor q_out, c10::optional<torch::Tensor> room) {
   const auto type = q.scalar_type();
   TORCH_CHECK(q.is_cuda(), "append: q must be on a GPU");
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf, "append: bf16 or fp16, got ", type_name(q));
@@ -443,6 +448,10 @@ void paged_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tens
               "append: table and lens slots differ");
   TORCH_CHECK(row_slot.numel() == rows && row_back.numel() == rows, "append: the plan has ", num(row_slot.numel()),
               " rows, q has ", num(rows));
+  if (room.has_value()) {
+    check_ints(*room, "append: room", q);
+    TORCH_CHECK(room->sizes() == lens.sizes(), "append: room must have one entry for each slot");
+  }
   AppendArgs a{};
   Width w(8);
   if (cos_t.has_value()) {
@@ -466,6 +475,7 @@ void paged_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tens
   a.lens = lens.data_ptr<int>();
   a.row_slot = row_slot.data_ptr<int>();
   a.row_back = row_back.data_ptr<int>();
+  a.room = room.has_value() ? room->data_ptr<int>() : nullptr;
   a.rows = int(rows);
   a.hq = int(q.size(1));
   a.hk = int(hk);

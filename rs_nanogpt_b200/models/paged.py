@@ -40,6 +40,7 @@ class PagedCache:
         self.table = torch.full((max_seqs, self.width), -1, **ints)
         self.lens = torch.zeros(max_seqs, **ints)
         self.refs = torch.zeros(pages, **ints)
+        self.room = torch.zeros(max_seqs, **ints)  # tokens granted and not yet written
 
     @property
     def state(self) -> paged.State:
@@ -50,13 +51,13 @@ class PagedCache:
 
     def grow(self, add) -> None:
         """Room for ``add[s]`` more tokens in every slot ``s``."""
-        paged.grow_pages(*self.state, self._list(add), self.page, out=self.state)
+        paged.grow_pages(*self.state, self._list(add), self.page, out=self.state, room=self.room)
 
     def fork(self, parents, children) -> None:
         paged.fork_pages(self.k, self.v, *self.state, self._list(parents), self._list(children), out=self.state)
 
     def free(self, seqs) -> None:
-        paged.free_pages(*self.state, self._list(seqs), out=self.state)
+        paged.free_pages(*self.state, self._list(seqs), out=self.state, room=self.room)
 
     def compact(self) -> None:
         paged.compact_pages(self.k, self.v, *self.state, out=self.state)
@@ -96,6 +97,7 @@ class PagedDecoder:
     def forward(self, ids: torch.Tensor, plan: paged.PrefixPlan) -> torch.Tensor:
         """``ids`` (rows,) int64 on the device: the new tokens of the plan's
         sequences, one sequence after another; the cache has grown by them.
+        Rows of a slot that could not grow are written nowhere (and reported).
         Returns the final normed hidden states (rows, C)."""
         cfg, st, cache = self.cfg, self.store, self.cache
         n, c, h, eps = ids.shape[0], cfg.n_embd, cfg.n_head, cfg.norm_eps
@@ -106,11 +108,12 @@ class PagedDecoder:
             qkv = gemm.linear(L.rmsnorm(x, eps), st.qkv_work(i))
             q, k, v = qkv.view(n, 3, h, cfg.head_dim).unbind(1)
             paged.append(q, k, v, cache.k[i], cache.v[i], cache.table, cache.lens, plan, self.cos, self.sin, qk_eps=eps,
-                         q_out=q)
+                         q_out=q, room=cache.room)
             paged.attention(q, cache.k[i], cache.v[i], cache.table, cache.lens, plan, out=y.view(n, h, cfg.head_dim))
             x = gemm.linear_residual(y, st.work_of(p + "attn.c_proj.weight"), x)
             a = gemm.linear_relu2_act(L.rmsnorm(x, eps), st.work_of(p + "mlp.c_fc.weight"))
             x = gemm.linear_residual(a, st.work_of(p + "mlp.c_proj.weight"), x)
+        cache.room.index_fill_(0, plan.row_slot.long(), 0)
         return L.rmsnorm(x, eps)
 
     @torch.no_grad()

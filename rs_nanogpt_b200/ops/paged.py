@@ -14,6 +14,14 @@ operators return ``(table, lens, refs)``; ``out`` takes three tensors for the
 result, which may be the inputs themselves (in place) and are fresh ones by
 default. No operator waits for the device: pages that run out or an index out
 of range are reported by ``kernel_status`` and the entry concerned is skipped.
+
+A fourth tensor, ``room`` (slots) int32, zero at first, keeps apart the tokens
+that ``grow_pages`` granted and those that are written: growing adds to it,
+``append`` writes no more of a slot's tokens than it says, and whoever has
+written a slot's tokens (into all layers) sets its entry to 0. It is optional;
+without it, an append after a growth that was refused writes over the last
+tokens that the cache holds, in pages that others may share, so the caller has
+to look at ``kernel_status`` in between.
 """
 from typing import Optional, Sequence, Tuple, Union
 
@@ -41,20 +49,22 @@ def fork_pages(k, v, table, lens, refs, parents, children, out: Optional[State] 
     return out
 
 
-def grow_pages(table, lens, refs, add, page: int, out: Optional[State] = None) -> State:
+def grow_pages(table, lens, refs, add, page: int, out: Optional[State] = None,
+               room: Optional[torch.Tensor] = None) -> State:
     """Make room for ``add[s]`` (int32, one a slot) more tokens in every slot:
     ``lens`` grows by it and missing pages are the lowest free ones, in the
     order of the slots. A slot whose pages are not to be had keeps its length
-    and is reported."""
+    and is reported. What is granted is added to ``room``."""
     out = _out(table, lens, refs, out)
-    ext().pages_grow(table, lens, refs, add, page, *out)
+    ext().pages_grow(table, lens, refs, add, page, *out, room)
     return out
 
 
-def free_pages(table, lens, refs, seqs, out: Optional[State] = None) -> State:
-    """Empty the slots ``seqs`` (int32); pages that nobody else holds are free."""
+def free_pages(table, lens, refs, seqs, out: Optional[State] = None, room: Optional[torch.Tensor] = None) -> State:
+    """Empty the slots ``seqs`` (int32); pages that nobody else holds are free.
+    The slots' entries of ``room`` become 0."""
     out = _out(table, lens, refs, out)
-    ext().pages_free(table, lens, refs, seqs, *out)
+    ext().pages_free(table, lens, refs, seqs, *out, room)
     return out
 
 
@@ -161,18 +171,21 @@ class PrefixPlan:
 
 
 def append(q, k, v, k_pages, v_pages, table, lens, plan: PrefixPlan, cos=None, sin=None, layout: str = "half",
-           qk_eps: Optional[float] = None, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+           qk_eps: Optional[float] = None, q_out: Optional[torch.Tensor] = None,
+           room: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Write the new tokens' keys and values into one layer's pages (pages, kv
     heads, rows of a page, head_dim), turned by their positions (``cos``,
     ``sin`` of ``rotary.tables``; none: not turned) and, with ``qk_eps``, each
     head of q and k divided by its root mean square as the model does after
     RoPE (rs-nanogpt src/model/attention.rs:68-116). ``lens`` counts the new
-    tokens already (``grow_pages`` comes first). Returns q, turned and normed
+    tokens already (``grow_pages`` comes first); with ``room``, tokens that it
+    did not grant are left out and reported. Returns q, turned and normed
     alike, in ``q_out`` (which may be q)."""
     if q_out is None:
         q_out = torch.empty_like(q)
     ext().paged_append(q, k, v, k_pages, v_pages, table, lens, plan.row_slot, plan.row_back, cos, sin,
-                       rotary.interleaved(layout), 0.0 if qk_eps is None else qk_eps, qk_eps is not None, q_out)
+                       rotary.interleaved(layout), 0.0 if qk_eps is None else qk_eps, qk_eps is not None, q_out,
+                       room)
     return q_out
 
 

@@ -81,3 +81,32 @@ def test_slots_outside_the_cache_are_refused(slots):
     with pytest.raises(ValueError):
         dec.feed([[1]] * len(slots), slots)
     assert _unchanged(dec, was)
+
+
+@gpu
+def test_appends_to_a_full_pool_change_nothing():
+    """A refused grow, used all the same: no page is written, of the slot or of those that share it."""
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    from rs_nanogpt_b200.ops._ext import kernel_status
+    kernel_status(True)
+    cfg, store = _store()
+    dec = PagedDecoder(store, pages=5, max_seqs=4, max_len=200, page=32)
+    dec.feed([_tokens(cfg, 64)], [0])
+    dec.cache.fork([0], [1])
+    dec.feed([_tokens(cfg, 96, 1)], [2])
+    was = _state(dec)
+    assert kernel_status(True) == 0
+    dec.cache.grow([0, 1, 0, 0])
+    assert kernel_status(True) == 6
+    dec.forward(torch.tensor([5], device="cuda"), dec.plan([(1, 0)], [1], [1]))
+    assert kernel_status(True) == 6 and _unchanged(dec, was)
+    # Reserved in two steps, written in one.
+    dec.cache.free([2])
+    dec.cache.grow([0, 1, 0, 0])
+    dec.cache.grow([0, 2, 0, 0])
+    new = _tokens(cfg, 3, 2)
+    dec.forward(torch.tensor(new, device="cuda"), dec.plan([(1, 0)], [3], [1]))
+    assert kernel_status(True) == 0
+    from rs_nanogpt_b200.models.reference import ReferenceGpt
+    ref = ReferenceGpt(store, torch.float32).forward(torch.tensor([_tokens(cfg, 64) + new + [9]], device="cuda"))[:, -1]
+    _close(dec.feed([[9]], [1]), ref)

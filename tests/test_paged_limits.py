@@ -1,0 +1,71 @@
+"""Paged cache operators at their limits: pages that run out, plans and tensors that do not fit,
+operands that lie over one another, values that a row may not see, states without entries."""
+import math
+import random
+
+import pytest
+import torch
+
+from test_paged import DEV, Batch, Model, _check_state, _i32, _pools, _state
+
+gpu = pytest.mark.gpu
+checked = pytest.mark.usefixtures("kernel_ok")
+
+
+# ---- pages that run out ------------------------------------------------------------------
+
+
+@gpu
+def test_refused_slots_keep_their_tokens():
+    """The append writes new tokens only: a slot whose growth was refused loses none of what it holds,
+    nor do those that share its pages."""
+    from rs_nanogpt_b200.ops import paged
+    from rs_nanogpt_b200.ops._ext import kernel_status
+    kernel_status(True)
+    page, d = 8, 64
+    k = torch.zeros(3, 1, page, d, device=DEV, dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    table, lens, refs = torch.full((4, 3), -1, device=DEV, dtype=torch.int32), _i32([0] * 4), _i32([0] * 3)
+    state, room = (table, lens, refs), _i32([0] * 4)
+
+    def new(slots, t, fill):
+        plan = paged.PrefixPlan([(len(slots), 0)], t, n_head=1, n_kv_head=1, head_dim=d, page=page, table_width=3,
+                                slots=slots)
+        x = torch.full((len(slots) * t, 1, d), float(fill), device=DEV, dtype=torch.bfloat16)
+        paged.append(x, x, x, k, v, table, lens, plan, room=room)
+        room[slots] = 0
+
+    paged.grow_pages(*state, _i32([8, 0, 5, 0]), page, out=state, room=room)
+    assert room.tolist() == [8, 0, 5, 0]
+    new([0], 8, 1)
+    new([2], 5, 2)
+    kk, vv = k.view(1, *k.shape), v.view(1, *v.shape)
+    paged.fork_pages(kk, vv, *state, _i32([0]), _i32([1]), out=state)  # a full page, shared
+    paged.grow_pages(*state, _i32([0, 0, 0, 8]), page, out=state, room=room)
+    new([3], 8, 3)
+    assert kernel_status(True) == 0
+    before = k.clone(), v.clone(), [x.clone() for x in state]
+    # No page is free: slots 0 and 1 are refused, slot 2 has room in its own page.
+    paged.grow_pages(*state, _i32([1, 2, 0, 0]), page, out=state, room=room)
+    assert kernel_status(True) == 6
+    paged.grow_pages(*state, _i32([0, 0, 1, 0]), page, out=state, room=room)
+    assert kernel_status(True) == 0 and lens.tolist() == [8, 8, 6, 8] and room.tolist() == [0, 0, 1, 0]
+    new([0, 2], 1, 9)
+    assert kernel_status(True) == 6
+    new([1], 2, 9)
+    assert kernel_status(True) == 6
+    own = int(table[2, 0])
+    assert (k[own, 0, 5] == 9).all()
+    for x, was in ((k, before[0]), (v, before[1])):
+        x[own, 0, 5] = 0
+        assert torch.equal(x, was)
+    # More rows than were granted: those that were not are left out.
+    paged.grow_pages(*state, _i32([0, 0, 1, 0]), page, out=state, room=room)
+    new([2], 3, 7)
+    assert kernel_status(True) == 6
+    assert (k[own, 0, 6] == 7).all() and (k[own, 0, 4] == 2).all()
+    # A slot that is freed has no room either.
+    paged.free_pages(*state, _i32([3]), out=state, room=room)
+    paged.grow_pages(*state, _i32([1, 0, 0, 0]), page, out=state, room=room)
+    paged.free_pages(*state, _i32([0]), out=state, room=room)
+    assert room.tolist() == [0] * 4 and kernel_status(True) == 0
