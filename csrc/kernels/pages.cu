@@ -83,14 +83,16 @@ __device__ __forceinline__ void copy_state(const PageState& s) {
   for (int i = gid; i < s.pages; i += all) s.refs[i] = s.refs_in[i];
 }
 
-// Exclusive sum over a CTA's threads; every thread also gets the total.
+// Exclusive sum over a CTA's threads; every thread also gets the total. Sums stop at
+// kMany, which is more than there can be pages or list entries, and are not exact there.
+constexpr int kMany = (1 << 30) - 1;
 __device__ __forceinline__ int cta_scan(int v, int* sm, int& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    if (lane >= o) x = min(x + y, kMany);
   }
   __syncthreads();  // sm may still be read from an earlier call
   if (lane == 31) sm[warp] = x;
@@ -100,7 +102,7 @@ __device__ __forceinline__ int cta_scan(int v, int* sm, int& total) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
+      if (lane >= o) w = min(w + y, kMany);
     }
     sm[lane] = w;
   }
@@ -214,7 +216,8 @@ __global__ void __launch_bounds__(kMetaThreads)
 
 // ---- grow ----------------------------------------------------------------------
 
-// ws list: free pages (pages).
+// ws lists: free pages (pages); of each slot, the first of its pages in that list
+// (slots; -1: refused), written only where there are too few pages for all.
 template <int C>
 __global__ void __launch_bounds__(kMetaThreads)
     grow_meta_kernel(const PageState s, const int* __restrict__ add, int* room, int* ws) {
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(kMetaThreads)
   using team = Team<C>;
   const int gid = team::gid();
   pdl_trigger();
-  int* spare = ws + kListAt;
+  int *spare = ws + kListAt, *served = spare + s.pages;
   copy_state<C>(s);
   int lo, hi, live;
   const int before = live_before<C>(s.refs_in, s.pages, sm, ws, lo, hi, live);
@@ -230,27 +233,50 @@ __global__ void __launch_bounds__(kMetaThreads)
     if (s.refs_in[p] <= 0) spare[f++] = p;
   team::sync();
   if (team::cta() != 0) return;
-  const int span = (s.slots + kMetaThreads - 1) / kMetaThreads;
+  const int span = (s.slots + kMetaThreads - 1) / kMetaThreads, avail = s.pages - live;
   const int i0 = min(s.slots, int(threadIdx.x) * span), i1 = min(s.slots, i0 + span);
+  auto pages_for = [&](int tokens) { return int((unsigned(tokens) + s.page - 1) / s.page); };
   auto need = [&](int i, int& len, int& have) {  // pages that slot i lacks; -1: it cannot be grown
     const int more = add[i];
     len = s.lens_in[i];
-    have = (len + s.page - 1) / s.page;
+    have = pages_for(len);
     if (more < 0 || len < 0 || long(len) + more > long(s.width) * s.page) return -1;
-    return (len + more + s.page - 1) / s.page - have;
+    return pages_for(len + more) - have;
   };
-  int mine = 0, total, len, have;
-  for (int i = i0; i < i1; ++i) mine += max(0, need(i, len, have));
-  int rank = cta_scan(mine, sm, total);
+  int len, have, mine = 0, total;
+  for (int i = i0; i < i1; ++i) mine = int(min(mine + unsigned(max(0, need(i, len, have))), unsigned(kMany)));
+  const int rank = cta_scan(mine, sm, total);
+  const bool enough = total <= avail;
+  if (!enough) {
+    // Served in order; a slot that wants more than is left takes nothing. A warp
+    // looks at 32 slots together and deals them their pages one by one.
+    if (threadIdx.x < 32) {
+      int used = 0;
+      for (int b = 0; b < s.slots; b += 32) {
+        const int i = b + int(threadIdx.x), m = i < s.slots ? max(0, need(i, len, have)) : 0;
+        int at = m ? -1 : 0;
+        for (unsigned left = __ballot_sync(0xffffffffu, m > 0); left; left &= left - 1) {
+          const int from = __ffs(left) - 1, want = __shfl_sync(0xffffffffu, m, from);
+          if (want > avail - used) continue;
+          if (int(threadIdx.x) == from) at = used;
+          used += want;
+        }
+        if (i < s.slots) served[i] = at;
+      }
+    }
+    __syncthreads();
+  }
+  int next = enough ? rank : 0;
   for (int i = i0; i < i1; ++i) {
-    const int m = need(i, len, have);
+    const int m = need(i, len, have), at = enough ? next : served[i];
+    next += max(0, m);
     if (m < 0) {
       report(s.err, kErrBounds);
-    } else if (rank + m > s.pages - live) {
+    } else if (at < 0) {
       report(s.err, kErrNoPages);  // this slot keeps its length
     } else {
       for (int e = 0; e < m; ++e) {
-        const int q = __ldcg(spare + rank + e);
+        const int q = __ldcg(spare + at + e);
         s.table[long(i) * s.width + have + e] = q;
         s.refs[q] = 1;
       }
@@ -259,7 +285,6 @@ __global__ void __launch_bounds__(kMetaThreads)
         if (room) room[i] += add[i];
       }
     }
-    rank += max(0, m);
   }
 }
 
@@ -515,7 +540,7 @@ void pages_grow(torch::Tensor table, torch::Tensor lens, torch::Tensor refs, tor
   check_int_vec(add, "grow_pages: add", table);
   TORCH_CHECK(add.sizes() == lens.sizes(), "grow_pages: add must have one entry for each slot");
   const at::cuda::CUDAGuard guard(table.device());
-  auto ws = workspace(table, s.pages);
+  auto ws = workspace(table, int64_t(s.pages) + s.slots);
   launch_team(s, "grow_pages", grow_meta_kernel<1>, grow_meta_kernel<kMetaCtas>, add.data_ptr<int>(),
               room_of(room, lens, "grow_pages"), ws.data_ptr<int>());
 }

@@ -53,8 +53,9 @@ def grow_pages(table, lens, refs, add, page: int, out: Optional[State] = None,
                room: Optional[torch.Tensor] = None) -> State:
     """Make room for ``add[s]`` (int32, one a slot) more tokens in every slot:
     ``lens`` grows by it and missing pages are the lowest free ones, in the
-    order of the slots. A slot whose pages are not to be had keeps its length
-    and is reported. What is granted is added to ``room``."""
+    order of the slots. A slot that lacks more pages than are left when its turn
+    comes keeps its length, is reported and takes nothing from those after it.
+    What is granted is added to ``room``."""
     out = _out(table, lens, refs, out)
     ext().pages_grow(table, lens, refs, add, page, *out, room)
     return out

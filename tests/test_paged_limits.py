@@ -69,3 +69,72 @@ def test_refused_slots_keep_their_tokens():
     paged.grow_pages(*state, _i32([1, 0, 0, 0]), page, out=state, room=room)
     paged.free_pages(*state, _i32([0]), out=state, room=room)
     assert room.tolist() == [0] * 4 and kernel_status(True) == 0
+
+
+@gpu
+def test_a_refused_slot_refuses_no_other():
+    """Slots are served in order; one that cannot be served takes nothing from those after it."""
+    from rs_nanogpt_b200.ops import paged
+    from rs_nanogpt_b200.ops._ext import kernel_status
+    kernel_status(True)
+    m = Model(2, 4, 3, 2)
+    m.grow([4, 1])
+    state = paged.grow_pages(*(x.to(DEV) for x in _state(m)), _i32([1, 1]), 4)  # slot 1 needs no page
+    assert kernel_status(True) == 6 and state[1].tolist() == [4, 2]
+    m = Model(3, 4, 8, 4)
+    m.grow([4, 0, 0, 0])
+    state = paged.grow_pages(*(x.to(DEV) for x in _state(m)), _i32([9, 2, 0, 4]), 4)
+    assert kernel_status(True) == 6
+    assert state[1].tolist() == [4, 2, 0, 4] and state[2].tolist() == [1, 1, 1]
+    assert state[0][:, 0].tolist() == [0, 1, -1, 2]
+
+
+def _grow_in_order(m, add):
+    """Model.grow where a refused slot takes nothing."""
+    free = [p for p, r in enumerate(m.refs) if r == 0]
+    refused = False
+    for s, a in enumerate(add):
+        if a < 0 or m.lens[s] + a > m.width * m.page:
+            continue
+        need = -(-(m.lens[s] + a) // m.page) - len(m.table[s])
+        if need > len(free):
+            refused = True
+            continue
+        for _ in range(need):
+            p = free.pop(0)
+            m.table[s].append(p)
+            m.refs[p] = 1
+        m.lens[s] += a
+    return refused
+
+
+@gpu
+@pytest.mark.parametrize("seed,pages,page,width,slots", [(0, 11, 4, 5, 7), (1, 90, 3, 6, 61), (2, 400, 2, 9, 1500),
+                                                         (3, 20000, 1, 40, 1100), (4, 5, 16, 3, 40)])
+def test_growing_past_the_pool(seed, pages, page, width, slots):
+    from rs_nanogpt_b200.ops import paged
+    from rs_nanogpt_b200.ops._ext import kernel_status
+    kernel_status(True)
+    rng = random.Random(seed)
+    m = Model(pages, page, width, slots)
+    state = tuple(x.to(DEV) for x in _state(m))
+    room, held = _i32([0] * slots), [0] * slots
+    refusals = 0
+    for _ in range(12):
+        most = max(1, 2 * pages * page // slots)
+        add = [rng.choice([0, 1, rng.randint(0, most)]) for _ in range(slots)]
+        add = [min(a, width * page - m.lens[s]) for s, a in enumerate(add)]
+        before = list(m.lens)
+        refused = _grow_in_order(m, add)
+        held = [h + n - b for h, n, b in zip(held, m.lens, before)]
+        state = paged.grow_pages(*state, _i32(add), page, out=state if rng.random() < 0.5 else None, room=room)
+        assert kernel_status(True) == (6 if refused else 0)
+        refusals += refused
+        _check_state(m, state)
+        assert room.tolist() == held
+        gone = rng.sample(range(slots), slots // 4)
+        m.free(gone)
+        held = [0 if s in set(gone) else h for s, h in enumerate(held)]
+        state = paged.free_pages(*state, _i32(gone), out=state if rng.random() < 0.5 else None, room=room)
+        assert room.tolist() == held
+    assert refusals
