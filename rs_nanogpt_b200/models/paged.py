@@ -128,10 +128,10 @@ class PagedDecoder:
         if min(slots) < 0 or max(slots) >= self.cache.lens.shape[0]:
             raise ValueError(f"feed: slots must be below {self.cache.lens.shape[0]}, got {list(slots)}")
         dev = self.store.device
+        plan = self.plan(groups or [(len(tokens), 0)], lens, slots)
         add = torch.zeros_like(self.cache.lens)
         add[torch.tensor(list(slots), device=dev)] = torch.tensor(lens, dtype=torch.int32, device=dev)
-        self.cache.grow(add)
-        plan = self.plan(groups or [(len(tokens), 0)], lens, slots)
+        self.cache.grow(add)  # after all checks: a refused call leaves the cache as it was
         hidden = self.forward(torch.tensor([t for s in tokens for t in s], dtype=torch.int64, device=dev), plan)
         last = torch.tensor(lens, device=dev).cumsum(0) - 1
         return gemm.linear(hidden[last], self.store.work_of("lm_head.weight"))

@@ -84,6 +84,20 @@ def test_slots_outside_the_cache_are_refused(slots):
 
 
 @gpu
+@checked
+def test_refused_arguments_leave_the_cache_as_it_was():
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    cfg, store = _store()
+    dec = PagedDecoder(store, pages=20, max_seqs=4, max_len=200, page=32)
+    dec.feed([_tokens(cfg, 64), _tokens(cfg, 40, 1)], [0, 1])
+    was = _state(dec)
+    for groups in ([(2, 33)], [(3, 0)], [(1, 0)], [(2, 32 * 100)], [(-1, 0), (3, 0)]):
+        with pytest.raises(ValueError):
+            dec.feed([[1], [2]], [0, 1], groups)
+        assert _unchanged(dec, was)
+
+
+@gpu
 def test_appends_to_a_full_pool_change_nothing():
     """A refused grow, used all the same: no page is written, of the slot or of those that share it."""
     from rs_nanogpt_b200.models.paged import PagedDecoder
