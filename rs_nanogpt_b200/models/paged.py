@@ -127,12 +127,15 @@ class PagedDecoder:
             raise ValueError("feed: one slot of its own and at least one token for each sequence")
         if min(slots) < 0 or max(slots) >= self.cache.lens.shape[0]:
             raise ValueError(f"feed: slots must be below {self.cache.lens.shape[0]}, got {list(slots)}")
+        ids = [t for s in tokens for t in s]
+        if min(ids) < 0 or max(ids) >= self.cfg.vocab_size:
+            raise ValueError(f"feed: token ids must be below the vocabulary's size, {self.cfg.vocab_size}")
         dev = self.store.device
         plan = self.plan(groups or [(len(tokens), 0)], lens, slots)
         add = torch.zeros_like(self.cache.lens)
         add[torch.tensor(list(slots), device=dev)] = torch.tensor(lens, dtype=torch.int32, device=dev)
         self.cache.grow(add)  # after all checks: a refused call leaves the cache as it was
-        hidden = self.forward(torch.tensor([t for s in tokens for t in s], dtype=torch.int64, device=dev), plan)
+        hidden = self.forward(torch.tensor(ids, dtype=torch.int64, device=dev), plan)
         last = torch.tensor(lens, device=dev).cumsum(0) - 1
         return gemm.linear(hidden[last], self.store.work_of("lm_head.weight"))
 

@@ -98,6 +98,20 @@ def test_refused_arguments_leave_the_cache_as_it_was():
 
 
 @gpu
+@checked
+def test_tokens_outside_the_vocabulary_are_refused():
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    cfg, store = _store()
+    dec = PagedDecoder(store, pages=20, max_seqs=4, max_len=200, page=32)
+    dec.feed([_tokens(cfg, 64), _tokens(cfg, 40, 1)], [0, 1])
+    was = _state(dec)
+    for ids in ([cfg.vocab_size], [-1], [1 << 40]):
+        with pytest.raises(ValueError):
+            dec.feed([[3], ids], [0, 1])
+        assert _unchanged(dec, was)
+
+
+@gpu
 def test_appends_to_a_full_pool_change_nothing():
     """A refused grow, used all the same: no page is written, of the slot or of those that share it."""
     from rs_nanogpt_b200.models.paged import PagedDecoder
