@@ -116,12 +116,25 @@ class PagedDecoder:
         cache.room.index_fill_(0, plan.row_slot.long(), 0)
         return L.rmsnorm(x, eps)
 
+    def _check_fits(self, slots: Sequence[int], new: Sequence[int]) -> None:
+        """Reads the cache's lengths and free pages: the growth that follows is granted whole."""
+        cache = self.cache
+        *held, free = torch.cat([cache.lens, (cache.refs <= 0).sum(dtype=torch.int32).view(1)]).tolist()
+        need = 0
+        for s, n in zip(slots, new):
+            if held[s] + n > self.max_len:
+                raise ValueError(f"feed: {held[s]} tokens in slot {s} and {n} new ones exceed max_len ({self.max_len})")
+            need += -(-(held[s] + n) // cache.page) - -(-held[s] // cache.page)
+        if need > free:
+            raise RuntimeError(f"paged cache: out of pages ({need} needed, {free} free)")
+
     @torch.no_grad()
     def feed(self, tokens: Sequence[Sequence[int]], slots: Sequence[int],
              groups: Optional[Sequence[Tuple[int, int]]] = None) -> torch.Tensor:
         """Append ``tokens[i]`` to the sequence in slot ``slots[i]``; ``groups``
         as in ``plan`` (none: nothing shared). Returns the (sequences, vocab)
-        bf16 logits of their last tokens."""
+        bf16 logits of their last tokens. Raises, and leaves the cache as it
+        was, where a sequence would pass ``max_len`` or the pages run out."""
         lens = [len(t) for t in tokens]
         if not lens or min(lens) == 0 or len(slots) != len(tokens) or len(set(slots)) != len(slots):
             raise ValueError("feed: one slot of its own and at least one token for each sequence")
@@ -132,6 +145,7 @@ class PagedDecoder:
             raise ValueError(f"feed: token ids must be below the vocabulary's size, {self.cfg.vocab_size}")
         dev = self.store.device
         plan = self.plan(groups or [(len(tokens), 0)], lens, slots)
+        self._check_fits(slots, lens)
         add = torch.zeros_like(self.cache.lens)
         add[torch.tensor(list(slots), device=dev)] = torch.tensor(lens, dtype=torch.int32, device=dev)
         self.cache.grow(add)  # after all checks: a refused call leaves the cache as it was

@@ -138,3 +138,29 @@ def test_appends_to_a_full_pool_change_nothing():
     from rs_nanogpt_b200.models.reference import ReferenceGpt
     ref = ReferenceGpt(store, torch.float32).forward(torch.tensor([_tokens(cfg, 64) + new + [9]], device="cuda"))[:, -1]
     _close(dec.feed([[9]], [1]), ref)
+
+
+@gpu
+@checked
+def test_feeds_that_do_not_fit_raise_and_change_nothing():
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    cfg, store = _store()
+    dec = PagedDecoder(store, pages=5, max_seqs=4, max_len=150, page=32)
+    dec.feed([_tokens(cfg, 64)], [0])
+    dec.cache.fork([0], [1])
+    dec.feed([_tokens(cfg, 70, 1)], [2])
+    was = _state(dec)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        dec.feed([[1], [2] * 27], [1, 2])
+    with pytest.raises(RuntimeError, match="out of pages"):
+        dec.feed([[1]], [1])
+    assert _unchanged(dec, was)
+    with pytest.raises(ValueError, match="max_len"):
+        dec.feed([[1] * 81], [2])
+    assert _unchanged(dec, was)
+    dec.feed([[2] * 26], [2])  # what fits is served
+    dec.cache.free([2])
+    dec.feed([[1] * 86], [1])  # up to max_len
+    assert dec.cache.lens.tolist() == [64, 150, 0, 0]
+    with pytest.raises(ValueError, match="max_len"):
+        dec.feed([[1]], [1])
