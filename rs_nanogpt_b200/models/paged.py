@@ -156,8 +156,8 @@ class PagedDecoder:
     @torch.no_grad()
     def sample_many(self, prompt: Sequence[int], n: int, max_new: int, temperature: float = 1.0, top_k: int = 50,
                     seed: int = 0, use_graph: bool = True) -> List[List[int]]:
-        """``n`` completions of ``max_new`` tokens of one prompt, in slots 0..n-1
-        of an empty cache (emptied again at the end). The prompt is prefilled
+        """``n`` completions of ``max_new`` tokens of one prompt, in slots 0..n-1,
+        which have to be empty (and are emptied again at the end). The prompt is prefilled
         once and forked; a decode step is one graph replay."""
         cache, dev, v = self.cache, self.store.device, self.cfg.vocab_size
         if not 0 < n <= cache.lens.shape[0] or max_new <= 0 or not prompt:
@@ -165,6 +165,8 @@ class PagedDecoder:
         if len(prompt) + max_new - 1 > self.max_len:
             raise ValueError(f"sample_many: prompt ({len(prompt)}) + {max_new} new tokens exceed max_len "
                              f"({self.max_len})")
+        if cache.lens[:n].any():
+            raise ValueError(f"sample_many: slots 0 to {n - 1} have to be empty")
         logits = self.feed([prompt], [0]).expand(n, v).contiguous()
         cache.fork([0] * (n - 1), list(range(1, n)))
         shared = len(prompt) // cache.page * cache.page

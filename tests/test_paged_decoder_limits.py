@@ -164,3 +164,22 @@ def test_feeds_that_do_not_fit_raise_and_change_nothing():
     assert dec.cache.lens.tolist() == [64, 150, 0, 0]
     with pytest.raises(ValueError, match="max_len"):
         dec.feed([[1]], [1])
+
+
+@gpu
+@checked
+def test_samples_need_empty_slots():
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    cfg, store = _store()
+    dec = PagedDecoder(store, pages=30, max_seqs=4, max_len=200, page=32)
+    alone = dec.sample_many(_tokens(cfg, 50), 2, 6, 1.0, 50, seed=1)
+    for used in (0, 1):
+        dec.feed([_tokens(cfg, 40, 3)], [used])
+        was = _state(dec)
+        with pytest.raises(ValueError, match="slot"):
+            dec.sample_many(_tokens(cfg, 50), 2, 6, 1.0, 50, seed=1)
+        assert _unchanged(dec, was)
+        dec.cache.free([used])
+    dec.feed([_tokens(cfg, 40, 3)], [3])  # another slot may be in use
+    assert dec.sample_many(_tokens(cfg, 50), 2, 6, 1.0, 50, seed=1) == alone
+    assert dec.cache.lens.tolist() == [0, 0, 0, 40]
