@@ -26,7 +26,8 @@ from .params import ParamStore
 class PagedCache:
     """Pages (layers, pages, kv heads, page, head_dim) for up to ``max_seqs``
     sequences of up to ``max_len`` tokens. All changes are made on the device
-    and in place; ``check`` (which waits for it) raises when pages ran out."""
+    and in place; ``check`` (which waits for the current stream) raises when
+    pages ran out."""
 
     def __init__(self, n_layer: int, n_kv_head: int, head_dim: int, pages: int, page: int, max_seqs: int, max_len: int,
                  dtype=torch.bfloat16, device="cuda"):
@@ -63,6 +64,7 @@ class PagedCache:
         paged.compact_pages(self.k, self.v, *self.state, out=self.state)
 
     def check(self) -> None:
+        torch.cuda.current_stream(self.table.device).synchronize()  # the status is read on the default stream
         status = kernel_status()
         if status == 6:
             raise RuntimeError("paged cache: out of pages")

@@ -183,3 +183,21 @@ def test_samples_need_empty_slots():
     dec.feed([_tokens(cfg, 40, 3)], [3])  # another slot may be in use
     assert dec.sample_many(_tokens(cfg, 50), 2, 6, 1.0, 50, seed=1) == alone
     assert dec.cache.lens.tolist() == [0, 0, 0, 40]
+
+
+@gpu
+def test_check_waits_for_the_stream_it_is_called_on():
+    from rs_nanogpt_b200.models.paged import PagedCache
+    from rs_nanogpt_b200.ops._ext import kernel_status
+    kernel_status(True)
+    cache = PagedCache(1, 1, 64, 2, 32, 2, 128)
+    add = torch.tensor([64, 32], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second or more
+        cache.grow(add)
+        with pytest.raises(RuntimeError, match="out of pages"):
+            cache.check()
+    torch.cuda.synchronize()
+    assert kernel_status(True) == 0
