@@ -85,7 +85,10 @@ class PagedDecoder:
         self.store, self.cfg, self.max_len = store, cfg, max_len
         self.cache = PagedCache(cfg.n_layer, cfg.n_head, cfg.head_dim, pages, page, max_seqs, max_len,
                                 device=store.device)
-        self.cos, self.sin = rotary.tables(cfg.head_dim, self.cache.width * page, cfg.rope_base, scaling, store.device)
+        # q and k are normed after the turn, so the scaling's factor on them goes into the scores.
+        self.cos, self.sin = rotary.tables(cfg.head_dim, self.cache.width * page, cfg.rope_base, scaling, store.device,
+                                           sharpen=False)
+        self.scale = cfg.head_dim ** -0.5 * (scaling.sharpening ** 2 if scaling else 1.0)
 
     def plan(self, groups: Sequence[Tuple[int, int]], q_lens,
              slots: Optional[Sequence[int]] = None) -> paged.PrefixPlan:
@@ -111,7 +114,8 @@ class PagedDecoder:
             q, k, v = qkv.view(n, 3, h, cfg.head_dim).unbind(1)
             paged.append(q, k, v, cache.k[i], cache.v[i], cache.table, cache.lens, plan, self.cos, self.sin, qk_eps=eps,
                          q_out=q, room=cache.room)
-            paged.attention(q, cache.k[i], cache.v[i], cache.table, cache.lens, plan, out=y.view(n, h, cfg.head_dim))
+            paged.attention(q, cache.k[i], cache.v[i], cache.table, cache.lens, plan, out=y.view(n, h, cfg.head_dim),
+                            scale=self.scale)
             x = gemm.linear_residual(y, st.work_of(p + "attn.c_proj.weight"), x)
             a = gemm.linear_relu2_act(L.rmsnorm(x, eps), st.work_of(p + "mlp.c_fc.weight"))
             x = gemm.linear_residual(a, st.work_of(p + "mlp.c_proj.weight"), x)

@@ -178,7 +178,8 @@ def append(q, k, v, k_pages, v_pages, table, lens, plan: PrefixPlan, cos=None, s
     heads, rows of a page, head_dim), turned by their positions (``cos``,
     ``sin`` of ``rotary.tables``; none: not turned) and, with ``qk_eps``, each
     head of q and k divided by its root mean square as the model does after
-    RoPE (rs-nanogpt src/model/attention.rs:68-116). ``lens`` counts the new
+    RoPE (rs-nanogpt src/model/attention.rs:68-116), which takes a factor common
+    to ``cos`` and ``sin`` out again (see ``rotary.Scaling``). ``lens`` counts the new
     tokens already (``grow_pages`` comes first); with ``room``, tokens that it
     did not grant are left out and reported. Returns q, turned and normed
     alike, in ``q_out`` (which may be q)."""

@@ -31,8 +31,11 @@ class Scaling:
     * ``"parts"``   pairs that turn more than ``high`` times over
       ``original_len`` positions keep their frequency, those that turn less than
       ``low`` times are slowed down by ``factor``, those between are blended;
-      cos and sin are multiplied by ``0.1 ln(factor) + 1``, which sharpens the
-      softmax as the context grows
+      cos and sin are multiplied by ``sharpening = 0.1 ln(factor) + 1``, which
+      sharpens the softmax as the context grows. A model that divides q and k
+      by their norm after the turn divides the factor away, too: it takes tables
+      with ``sharpen=False`` and multiplies the attention's scale by
+      ``sharpening ** 2``
     """
     kind: str
     factor: float
@@ -48,16 +51,21 @@ class Scaling:
         if self.kind == "parts" and not (self.original_len > 0 and self.low < self.high):
             raise ValueError("rotary scaling by parts needs original_len > 0 and low < high")
 
+    @property
+    def sharpening(self) -> float:
+        return 0.1 * math.log(self.factor) + 1.0 if self.kind == "parts" else 1.0
+
 
 def tables(rot: int, positions: int, base: float = 10000.0, scaling: Optional[Scaling] = None,
-           device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
-    """cos and sin, fp32 ``(positions, rot / 2)``. Angles are formed in 64 bits:
+           device="cuda", sharpen: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin, fp32 ``(positions, rot / 2)``, multiplied by the scaling's
+    ``sharpening`` unless ``sharpen`` is false. Angles are formed in 64 bits:
     in 32 bits the angle of position 100000 is off by up to 0.004 radians."""
     if rot <= 0 or rot % 2:
         raise ValueError(f"rotary: rot must be even and positive, got {rot}")
     if positions <= 0:
         raise ValueError(f"rotary: positions must be positive, got {positions}")
-    mul = 1.0
+    mul = scaling.sharpening if scaling is not None and sharpen else 1.0
     if scaling is not None and scaling.kind == "ntk":
         if rot == 2:
             raise ValueError("rotary: ntk scaling needs more than one pair")
@@ -69,7 +77,6 @@ def tables(rot: int, positions: int, base: float = 10000.0, scaling: Optional[Sc
         turns = scaling.original_len * w / (2 * math.pi)
         keep = ((turns - scaling.low) / (scaling.high - scaling.low)).clamp_(0, 1)
         w = w * (keep + (1 - keep) / scaling.factor)
-        mul = 0.1 * math.log(scaling.factor) + 1.0
     angle = torch.outer(torch.arange(positions, device=device, dtype=torch.float64), w)
     return (angle.cos() * mul).float(), (angle.sin() * mul).float()
 

@@ -186,6 +186,39 @@ def test_samples_need_empty_slots():
 
 
 @gpu
+@checked
+@pytest.mark.parametrize("kind", ["parts", "linear"])
+def test_scaling_sharpens_behind_the_norm(kind, monkeypatch):
+    """Frequencies scaled by parts multiply the scores by (0.1 ln(factor) + 1)^2, although the norm of q and k
+    divides a common factor of theirs away."""
+    from rs_nanogpt_b200.models.paged import PagedDecoder
+    from rs_nanogpt_b200.ops import paged, rotary
+    cfg, store = _store(seq=128)
+    f = 16.0
+    dec = PagedDecoder(store, 20, 2, 300, page=32, scaling=rotary.Scaling(kind, f, original_len=128))
+    calls, attention = [], paged.attention
+
+    def spy(q, k, v, *args, **kw):
+        q = q.clone()
+        out = attention(q, k, v, *args, **kw)
+        calls.append((q, k.clone(), v.clone(), out.clone()))
+        return out
+
+    monkeypatch.setattr(paged, "attention", spy)
+    x = _tokens(cfg, 250)
+    dec.feed([x], [0])
+    table, mul = dec.cache.table[0].long(), 0.1 * math.log(f) + 1 if kind == "parts" else 1.0
+    for q, k, v, out in calls:
+        # Unit root mean square: nothing of the factor is left in q and k.
+        assert (q.double().square().mean(-1) - 1).abs().max() < 0.02
+        k, v = (y[table[:8]].transpose(0, 1).flatten(1, 2)[:, :250].double() for y in (k, v))
+        z = torch.einsum("qhd,hkd->hqk", q.double(), k) * (mul * mul / math.sqrt(cfg.head_dim))
+        z.masked_fill_(torch.ones(250, 250, device="cuda", dtype=torch.bool).triu(1), -math.inf)
+        ref = torch.einsum("hqk,hkd->qhd", torch.softmax(z, -1), v)
+        assert (out.double() - ref).abs().max() <= (2 * 2.0 ** -8 + 4e-4) * v.abs().max()
+
+
+@gpu
 def test_check_waits_for_the_stream_it_is_called_on():
     from rs_nanogpt_b200.models.paged import PagedCache
     from rs_nanogpt_b200.ops._ext import kernel_status
