@@ -507,11 +507,11 @@ void launch(const torch::Tensor& k, const torch::Tensor& v, const Args& a, const
 // q, out: (rows, query heads, head_dim); k, v: one layer's pages (pages, kv heads,
 // rows of a page, head_dim). items, big_items: (n, 8) int32; shared_item, own_item:
 // item of each (row, query head of a kv head), plus kBig for big items, -1 where
-// there is none.
+// there is none. plan_page: rows of the pages that the items were made for.
 void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                      torch::Tensor items, torch::Tensor big_items, torch::Tensor slot_of_seq, torch::Tensor row_slot,
                      torch::Tensor row_back, torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot,
-                     double scale, torch::Tensor out, c10::optional<torch::Tensor> lse) {
+                     int64_t plan_page, double scale, torch::Tensor out, c10::optional<torch::Tensor> lse) {
   using namespace pa;
   const auto type = q.scalar_type();
   TORCH_CHECK(q.is_cuda(), "paged_attention: q must be on a GPU");
@@ -536,6 +536,10 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   TORCH_CHECK(hk > 0 && hq % hk == 0, "paged_attention: ", num(hq), " query heads on ", num(hk), " kv heads");
   TORCH_CHECK(page >= 8 && (page & (page - 1)) == 0 && page <= 4096,
               "paged_attention: rows of a page must be a power of two from 8 to 4096, got ", num(page));
+  // Runs begin where a page of the plan does; inside one of another size a box of
+  // keys would run on into the next head.
+  TORCH_CHECK(page == plan_page, "paged_attention: the plan is for pages of ", num(plan_page), " rows, these have ",
+              num(page));
   for (const auto* t : {&table, &lens, &items, &big_items, &slot_of_seq, &row_slot, &row_back, &shared_item, &own_item})
     TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
                 "paged_attention: table, lens and the plan must be contiguous int32 on ", place(q));

@@ -202,6 +202,6 @@ def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[
     if out is None:
         out = torch.empty_like(q)
     ext().paged_attention(q, k_pages, v_pages, table, lens, plan.items, plan.big_items, plan.slot_of_seq, plan.row_slot,
-                          plan.row_back, plan.shared_item, plan.own_item, plan.max_slot,
+                          plan.row_back, plan.shared_item, plan.own_item, plan.max_slot, plan.page,
                           q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
     return out

@@ -138,3 +138,19 @@ def test_growing_past_the_pool(seed, pages, page, width, slots):
         state = paged.free_pages(*state, _i32(gone), out=state if rng.random() < 0.5 else None, room=room)
         assert room.tolist() == held
     assert refusals
+
+
+# ---- plans and operands that do not fit ------------------------------------------------------
+
+
+@gpu
+@checked
+def test_a_plan_for_other_pages_is_refused():
+    from rs_nanogpt_b200.ops import paged
+    b = Batch([(30, 64)], [5] * 30, 1, 4, 2, 64, 32, torch.bfloat16)
+    b.run()
+    for page in (8, 16, 64):
+        b.plan = paged.PrefixPlan([(30, 64)], 1, n_head=4, n_kv_head=2, head_dim=64, page=page,
+                                  table_width=b.table.shape[1] * 32 // page)
+        with pytest.raises(RuntimeError, match="page"):
+            b.run()
