@@ -35,6 +35,7 @@
 #include "flash_common.cuh"
 #include "launch.h"
 #include "message.h"
+#include "overlap.h"
 #include "paged_attn.cuh"
 #include "status.h"
 #include "tma_host.h"
@@ -524,6 +525,7 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
     TORCH_CHECK(t->stride(2) == 1 && t->stride(0) % 2 == 0 && t->stride(1) % 2 == 0 &&
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 4 == 0,
                 "paged_attention: rows and heads of q and out must be 4-byte aligned, elements contiguous");
+  check_result(Operand(q, "paged_attention: q"), Operand(out, "paged_attention: out"));
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(),
               "paged_attention: pages must be (pages, kv heads, rows, head_dim)");
   for (const auto* t : {&k, &v}) {

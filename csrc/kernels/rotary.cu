@@ -19,6 +19,7 @@
 
 #include "common.cuh"
 #include "message.h"
+#include "overlap.h"
 #include "status.h"
 
 namespace nk {
@@ -305,24 +306,6 @@ Heads heads_of(const torch::Tensor& src, const torch::Tensor& dst) {
   return Heads{src.data_ptr(), dst.data_ptr(), src.stride(0), src.stride(1), dst.stride(0), dst.stride(1)};
 }
 
-// In place, or to memory of its own: a shifted copy over itself is refused.
-void check_alias(const torch::Tensor& src, const torch::Tensor& dst, const char* name) {
-  if (src.numel() == 0 || (src.data_ptr() == dst.data_ptr() && src.strides() == dst.strides())) return;
-  auto end = [](const torch::Tensor& t) {
-    int64_t n = 1;
-    for (int i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-    return static_cast<const char*>(t.data_ptr()) + n * t.element_size();
-  };
-  // Column blocks of one buffer (q and k of a fused projection) interleave without
-  // overlapping: equal row strides, and starts further apart than a row's elements.
-  const char *s0 = static_cast<const char*>(src.data_ptr()), *d0 = static_cast<const char*>(dst.data_ptr());
-  if (s0 >= end(dst) || d0 >= end(src)) return;
-  const int64_t es = src.element_size(), row = src.stride(0) * es;
-  const int64_t span = ((src.size(1) - 1) * src.stride(1) + src.size(2)) * es;
-  const int64_t gap = s0 > d0 ? s0 - d0 : d0 - s0;
-  TORCH_CHECK(src.stride(0) == dst.stride(0) && gap >= span && gap + span <= row, name, ": overlaps its output");
-}
-
 template <typename T>
 void launch_rotate(const RotateArgs& a, int64_t v, unsigned grid, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
@@ -369,8 +352,15 @@ void rotate(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor pos, 
   check_tables(cos_t, sin_t, q, d);
   check_ints(pos, "rotate: pos", q);
   TORCH_CHECK(pos.dim() == 1 && pos.size(0) == rows, "rotate: pos must have ", num(rows), " entries");
-  check_alias(q, q_out, "rotate: q");
-  if (k.has_value()) check_alias(*k, *k_out, "rotate: k");
+  const Operand oq(q, "rotate: q"), oq_out(q_out, "rotate: q_out");
+  check_result(oq, oq_out);
+  if (k.has_value()) {
+    const Operand ok(*k, "rotate: k"), ok_out(*k_out, "rotate: k_out");
+    check_result(ok, ok_out);
+    check_disjoint(oq_out, ok);
+    check_disjoint(ok_out, oq);
+    check_disjoint(oq_out, ok_out);
+  }
   RotateArgs a{};
   a.hq = int(q.size(1));
   a.heads = a.hq + (k.has_value() ? int(k->size(1)) : 0);
@@ -431,7 +421,10 @@ void paged_append(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tens
   check_heads(v, "append: v", q, rows, d);
   check_heads(q_out, "append: q_out", q, rows, d);
   TORCH_CHECK(v.size(1) == hk && q_out.size(1) == q.size(1), "append: head counts of k and v, q and q_out differ");
-  check_alias(q, q_out, "append: q");
+  const Operand oq_out(q_out, "append: q_out");
+  check_result(Operand(q, "append: q"), oq_out);
+  check_disjoint(oq_out, Operand(k, "append: k"));
+  check_disjoint(oq_out, Operand(v, "append: v"));
   for (const auto* p : {&k_pages, &v_pages}) {
     TORCH_CHECK(p->device() == q.device() && p->scalar_type() == type && p->dim() == 4 && p->size(1) == hk &&
                     p->size(3) == d && p->sizes() == k_pages.sizes(),

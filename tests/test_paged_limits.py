@@ -154,3 +154,55 @@ def test_a_plan_for_other_pages_is_refused():
                                   table_width=b.table.shape[1] * 32 // page)
         with pytest.raises(RuntimeError, match="page"):
             b.run()
+
+
+@gpu
+@checked
+def test_outputs_over_other_operands_are_refused():
+    from rs_nanogpt_b200.ops import paged, rotary
+    n, h, d = 6, 2, 64
+    cos, sin = rotary.tables(32, 64)
+    pos = torch.arange(n, device=DEV, dtype=torch.int32)
+    buf = torch.randn(8 * n * h * d, device=DEV).bfloat16()
+
+    def block(at, heads=h):
+        return buf[at * d:at * d + n * heads * d].view(n, heads, d)
+
+    q, k, far, far2 = block(0), block(n * h), block(2 * n * h), block(3 * n * h)
+    wide = buf[:n * d].view(n, 1, d).expand(n, h, d)
+    for args in [dict(q_out=k, k_out=far), dict(q_out=far, k_out=q), dict(q_out=far, k_out=far),
+                 dict(q_out=block(n * h + 1), k_out=far), dict(q_out=far, k_out=block(2 * n * h + h)),
+                 dict(q_out=wide, k_out=far), dict(q_out=k, k_out=k), dict(q_out=far, k_out=wide)]:
+        before = buf.clone()
+        with pytest.raises(RuntimeError):
+            rotary.rotate(q, k, pos, cos, sin, **args)
+        assert torch.equal(buf, before)
+    with pytest.raises(RuntimeError):
+        rotary.rotate(q, q, pos, cos, sin, q_out=q, k_out=q)
+    # What shares a buffer without lying over one another is served: column blocks of a row, heads in turn,
+    # heads before rows, one after another.
+    fused = torch.randn(n, 3, h, d, device=DEV).bfloat16()
+    turns = torch.randn(n, h, 3, d, device=DEV).bfloat16()
+    first = torch.randn(3, h, n, d, device=DEV).bfloat16().permute(2, 0, 1, 3)
+    ragged = torch.randn(n, 7 * d, device=DEV).bfloat16()
+    for a, b in [(fused[:, 0], fused[:, 1]), (fused[:, 2], fused[:, 0]), (turns[:, :, 0], turns[:, :, 2]),
+                 (first[:, 0], first[:, 1]), (ragged[:, 2 * d:].view(n, 5, d), ragged[:, :2 * d].view(n, 2, d)),
+                 (ragged[:1, d:2 * d].view(1, 1, d), ragged[:1, 2 * d:4 * d].view(1, 2, d)), (q, k), (q, q)]:
+        want = rotary.rotate(a.clone(), b.clone(), pos[:len(a)], cos, sin)
+        got = rotary.rotate(a, b, pos[:len(a)], cos, sin, q_out=far, k_out=far2) if a is b else rotary.rotate(
+            a, b, pos[:len(a)], cos, sin, q_out=a, k_out=b)
+        for x, y in zip(want, got):  # up to a step of the type, where another alignment orders the products otherwise
+            assert ((x.float() - y.float()).abs() <= x.float().abs() * 2.0 ** -7).all()
+    # The append and the attention.
+    c = Batch([(1, 0)], [n], n, h, h, d, 32, torch.bfloat16)
+    kp, vp, t, lens = c.k.to(DEV), c.v.to(DEV), c.dev_table, c.dev_lens
+    for args in [(q, k, far, k), (q, k, far, far), (q, k, far, block(n * h + 1)), (q, k, far, wide)]:
+        with pytest.raises(RuntimeError):
+            paged.append(*args[:3], kp, vp, t, lens, c.plan, q_out=args[3])
+    paged.append(fused[:, 0], fused[:, 1], fused[:, 2], kp, vp, t, lens, c.plan, q_out=fused[:, 0])
+    with pytest.raises(RuntimeError):
+        paged.attention(q, kp, vp, t, lens, c.plan, out=block(1))
+    with pytest.raises(RuntimeError):
+        paged.attention(q, kp, vp, t, lens, c.plan, out=wide)
+    want = paged.attention(q, kp, vp, t, lens, c.plan)
+    assert torch.equal(paged.attention(q, kp, vp, t, lens, c.plan, out=q), want)
