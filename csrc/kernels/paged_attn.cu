@@ -351,15 +351,89 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_wait();  // started beside the kernel of the big items: it ends, and the join begins, after that one
 }
 
+// The output of one (row, query head) from the keys that it sees and no others, key by
+// key in fp32; by L lanes. The tensor cores multiply the probabilities of a tile with
+// the values of all its keys, so a NaN or an infinite value of a key that other rows of
+// the tile see comes out as 0 * inf = NaN in rows that do not see it. Those rows are
+// done again here; no call comes here where values are finite, and no row whose runs
+// hold no key that it does not see.
+template <typename T, int D, int L>
+__device__ __noinline__ void attend_alone(const Args& a, const int* shared_item, const int* own_item, int id) {
+  const unsigned lanes = (L == 32 ? 0xffffffffu : (1u << (L % 32)) - 1) << (threadIdx.x % 32 / L * L);
+  const int hq = a.hk * a.share, row = id / hq, h = id % hq, pair = row * a.share + h % a.share;
+  const int slot = a.row_slot[row], len = length_of(a, slot), keys = len - a.row_back[row];
+  const int own = own_item[pair], shared = shared_item[pair];
+  auto item = [&](int i) -> const Item& { return (i >= kBig ? a.work[1] : a.work[0]).items[i & (kBig - 1)]; };
+  if (keys >= len - item(own).keys && (shared < 0 || keys >= item(shared).key0 + item(shared).keys)) return;
+  constexpr int E = D / L, U = 4, W = E < 4 ? E : 4;  // element e of a lane: as in the join
+  const int c0 = threadIdx.x % L * W, head = h / a.share;
+  auto load = [](const T* p, float(&x)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 w = unpack<T>(*reinterpret_cast<const uint32_t*>(p + (e / W) * W * L + e % W));
+      x[e] = w.x;
+      x[e + 1] = w.y;
+    }
+  };
+  float q[E], o[E], m = -INFINITY, l = 0.f;
+  load(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head + c0, q);
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < keys; j += U) {
+    float s[U], v[U][E], mx = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = min(j + u, keys - 1), page = a.table[long(slot) * a.width + key / a.page];
+      const int pg = page < 0 || page >= a.pages ? 0 : page;  // as the other kernels, which report it
+      const long at = long(head * a.page + key % a.page) * D + c0;
+      float k[E];
+      load(static_cast<const T*>(a.k) + pg * a.k_page + at, k);
+      load(static_cast<const T*>(a.v) + pg * a.v_page + at, v[u]);
+      s[u] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[u] = fmaf(q[e], k[e], s[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int b = L / 2; b > 0; b >>= 1) s[u] += __shfl_xor_sync(lanes, s[u], b);
+      s[u] *= a.sl2;
+      mx = fmaxf(mx, s[u]);
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx, alpha = exp2f(m - ref);
+    m = mx;
+    l *= alpha;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= alpha;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j + u >= keys) break;
+      const float p = exp2f(s[u] - ref);
+      l += p;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(p, v[u][e], o[e]);
+    }
+  }
+  const float inv = inverse(l);
+  T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + c0;
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + (e / W) * W * L + e % W) = pack<T>(o[e] * inv, o[e + 1] * inv);
+}
+
 // Joins the partials of every (row, query head) that the kernels above left in
 // several pieces: L lanes each. A lane looks up one partial, so their loads are in
 // flight together, and the outputs are added with the weights known. All 32 lanes
 // where there are few pairs and so many partials of each (latency counts), eight
 // where there are many pairs of few partials (loads in flight count).
 constexpr int kJoinThreads = 128;
+// The CTAs an SM keep the registers at what the join itself needs: attend_alone, which
+// hardly any call reaches, may spill.
 template <typename T, int D, int L>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, const int* __restrict__ shared_item,
-                                                                  const int* __restrict__ own_item) {
+__global__ void __launch_bounds__(kJoinThreads, D == 128 && L == 8 ? 7 : 9)
+    paged_join_kernel(const __grid_constant__ Args a, const int* __restrict__ shared_item,
+                      const int* __restrict__ own_item) {
   constexpr int E = D / L, U = 4 * L / 32 + 1, W = E < 4 ? E : 4;  // W: floats of a load
   const int id = (blockIdx.x * kJoinThreads + threadIdx.x) / L, lane = threadIdx.x % L;
   const unsigned lanes = (L == 32 ? 0xffffffffu : (1u << (L % 32)) - 1) << (threadIdx.x % 32 / L * L);
@@ -368,6 +442,15 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
   const int row = id / hq, h = id % hq, head = h / a.share, pair = row * a.share + h % a.share;
   const int item[2] = {own_item[pair], shared_item[pair]};  // the plan's: no kernel before this one writes them
   pdl_wait();
+  // The output that a pair's only piece may have written, on its way with the look-ups.
+  T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + lane * W;
+  uint32_t* word[E / 2];
+  uint32_t written[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    word[e / 2] = reinterpret_cast<uint32_t*>(dst + (e / W) * W * L + e % W);
+    if (item[1] < 0) written[e / 2] = *word[e / 2];
+  }
   // Partials of either run: the first at its base slot, the others worker by worker.
   int count[2] = {0, 0}, c0[2];
 #pragma unroll
@@ -381,7 +464,16 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
     count[s] = (u + n - 1) / size - c0[s] + 1;
   }
   const int parts = count[0] + count[1];
-  if (parts == 1 && (item[0] < 0 || item[1] < 0)) return;  // its only piece wrote the output
+  bool nan = false;
+  if (parts == 1 && (item[0] < 0 || item[1] < 0)) {  // its only piece wrote the output
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      const float2 x = unpack<T>(written[e]);
+      nan |= isnan(x.x) || isnan(x.y);
+    }
+    if (__any_sync(lanes, nan)) attend_alone<T, D, L>(a, shared_item, own_item, id);
+    return;
+  }
   float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
@@ -445,11 +537,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
     }
   }
   const float inv = inverse(l);
-  T* dst = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + lane * W;
 #pragma unroll
-  for (int e = 0; e < E; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + (e / W) * W * L + e % W) = pack<T>(o[e] * inv, o[e + 1] * inv);
+  for (int e = 0; e < E; e += 2) {
+    nan |= isnan(o[e]) || isnan(o[e + 1]);
+    *word[e / 2] = pack<T>(o[e] * inv, o[e + 1] * inv);
+  }
   if (a.lse && lane == 0) a.lse[long(row) * hq + h] = lse_of(m, l);
+  if (__any_sync(lanes, nan) && !isnan(l)) attend_alone<T, D, L>(a, shared_item, own_item, id);
 }
 
 CUtensorMap page_map(const torch::Tensor& t, int most_rows, const char* name) {
@@ -563,10 +657,15 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   }
   if (rows == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
+  if (out.data_ptr() == q.data_ptr()) q = q.clone();  // the join may need q again when out is written
   Args a{};
   a.q = q.data_ptr();
   a.q_row = q.stride(0);
   a.q_head = q.stride(1);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_page = k.stride(0);
+  a.v_page = v.stride(0);
   a.table = table.data_ptr<int>();
   a.lens = lens.data_ptr<int>();
   a.width = int(table.size(1));

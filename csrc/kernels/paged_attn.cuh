@@ -56,6 +56,8 @@ struct Args {
   long out_row, out_head;
   float* lse;        // may be null
   int* err;
+  const void *k, *v;     // the pages, beside the tensor maps of them
+  long k_page, v_page;   // elements
 };
 
 // mbar_wait that polls for a while before it first reads the timer, which would
@@ -228,6 +230,15 @@ template <>
 __device__ __forceinline__ uint32_t pack<__half>(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) { return unpack_bf16x2(w); }
+template <>
+__device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 // Items of many rows, on tcgen05 (paged_attn_tc.cu). The map's boxes are

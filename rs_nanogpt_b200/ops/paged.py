@@ -196,7 +196,8 @@ def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[
     """Causal attention of the new tokens ``q`` (rows, heads, head_dim) over one
     layer's pages, the keys that a group shares read once for all its rows.
     ``lens`` counts the new tokens; the last of them sees all of its sequence. A
-    row without keys (an empty slot) gives 0. ``lse`` (rows, heads) fp32 takes
+    row without keys (an empty slot) gives 0. A NaN or infinite value reaches
+    the rows that see its key and no others. ``out`` may be q. ``lse`` (rows, heads) fp32 takes
     the log of each row's softmax sum (-inf without keys). ``scale`` is
     1 / sqrt(head_dim) by default."""
     if out is None:

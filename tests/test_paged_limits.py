@@ -206,3 +206,66 @@ def test_outputs_over_other_operands_are_refused():
         paged.attention(q, kp, vp, t, lens, c.plan, out=wide)
     want = paged.attention(q, kp, vp, t, lens, c.plan)
     assert torch.equal(paged.attention(q, kp, vp, t, lens, c.plan, out=q), want)
+
+
+# ---- what a row may not see ------------------------------------------------------------------
+
+
+HIDDEN = {
+    # groups, tails, new tokens, hq, hk, d, page; (sequence, token, element, value) of the values' first kv head
+    "a short turn": ([(1, 0)], [40], [40], 1, 1, 64, 16, [(0, 20, 3, math.nan), (0, 33, 9, math.inf)]),
+    "heads of one": ([(1, 0), (1, 0)], [30, 9], [5, 1], 4, 2, 128, 32, [(0, 27, 0, -math.inf), (1, 8, 127, math.nan)]),
+    "a long turn": ([(1, 0)], [300], [300], 2, 1, 128, 64, [(0, 150, 5, math.nan), (0, 299, 90, math.inf)]),
+    "turns behind a prefix": ([(3, 128)], [70, 200, 33], [70, 150, 33], 4, 2, 64, 16,
+                              [(0, 190, 1, math.nan), (1, 300, 2, math.inf), (2, 140, 63, math.nan)]),
+    "a turn in parts": ([(1, 0)], [12000], [60], 2, 1, 64, 64, [(0, 11970, 5, math.nan), (0, 11999, 6, -math.inf)]),
+    "a few tokens in parts": ([(1, 0)], [6000], [8], 2, 1, 64, 64, [(0, 5994, 31, math.nan), (0, 5999, 2, math.inf)]),
+    "a long turn in parts": ([(1, 0)], [9000], [200], 4, 4, 128, 128, [(0, 8900, 100, math.nan)]),
+    "many samples": ([(40, 512)], [1 + i for i in range(40)], 1, 8, 1, 128, 64,
+                     [(3, 515, 17, math.nan), (0, 7, 20, math.inf)]),
+}
+
+
+@gpu
+@checked
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", HIDDEN)
+def test_values_that_a_row_does_not_see_do_not_reach_it(name, dtype):
+    """A NaN or infinite value reaches the rows that see its key and no other, of the same tile and before it."""
+    groups, tails, q_lens, hq, hk, d, page, bad = HIDDEN[name]
+    b = Batch(groups, tails, q_lens, hq, hk, d, page, dtype)
+    for s, at, e, x in bad:
+        b.v[int(b.table[s, at // page]), 0, at % page, e] = x
+    lse = torch.empty(b.q.shape[:2], device=DEV)
+    scale = 1 / math.sqrt(d)
+    out = b.run(lse=lse).double().cpu()
+    ref, ref_lse = b.reference(scale)
+    assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(out.isinf(), ref.isinf())
+    assert ref.isnan().any() or ref.isinf().any()
+    ok = ref.isfinite()
+    unit = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    vmax = b.v[torch.isfinite(b.v)].abs().max().item()
+    # As for finite values: P and the output are rounded to the type, scores are off by less than 2e-4.
+    assert (out - ref)[ok].abs().max() <= (2 * unit + 4e-4) * vmax
+    assert (lse.double().cpu() - ref_lse).abs().max() <= 2e-4
+    from rs_nanogpt_b200.ops import paged
+    q = b.q.to(DEV)
+    paged.attention(q, b.k.to(DEV), b.v.to(DEV), b.dev_table, b.dev_lens, b.plan, out=q)
+    assert torch.equal(q.double().cpu().nan_to_num(7.0), out.nan_to_num(7.0))
+
+
+@gpu
+@checked
+def test_members_shorter_than_the_prefix_do_not_see_its_end():
+    b = Batch([(4, 192)], [9, 30, 1, 5], 1, 4, 4, 128, 64, torch.bfloat16)
+    b.v[int(b.table[0, 1]), 0, 40, 11] = math.nan  # token 104 of the shared pages
+    b.v[int(b.table[0, 2]), 1, 3, 12] = math.inf   # token 131
+    for lens in ([70, 222, 193, 104], [104, 105, 131, 132]):
+        b.lens = lens
+        b.dev_lens = _i32(lens)
+        out = b.run().double().cpu()
+        ref, _ = b.reference(1 / math.sqrt(128))
+        assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(out.isinf(), ref.isinf())
+        ok = ref.isfinite()
+        vmax = b.v[torch.isfinite(b.v)].abs().max().item()
+        assert (out - ref)[ok].abs().max() <= (2 * 2.0 ** -8 + 4e-4) * vmax
