@@ -24,6 +24,7 @@
 #include <torch/extension.h>
 
 #include <climits>
+#include <utility>
 
 #include "common.cuh"
 #include "launch.h"
@@ -52,6 +53,7 @@ struct PageState {
   const int *table_in, *lens_in, *refs_in;
   int *table, *lens, *refs;
   int slots, width, pages, page;  // page: rows of one
+  bool fresh;                     // the outputs are other tensors than the inputs
   int* err;
 };
 
@@ -61,12 +63,10 @@ constexpr int kWsCounts = 0, kWsPairs = 8, kListAt = 16;
 
 __device__ __forceinline__ void report(int* err, int code) { atomicCAS(err, 0, code); }
 
-__device__ __forceinline__ bool copies(const PageState& s) { return s.table != s.table_in; }
-
 // table, lens and refs into the outputs, by the whole team.
 template <int C>
 __device__ __forceinline__ void copy_state(const PageState& s) {
-  if (!copies(s)) return;
+  if (!s.fresh) return;
   constexpr int all = Team<C>::kAll, U = 4;
   const int gid = Team<C>::gid();
   const long n = long(s.slots) * s.width;
@@ -427,15 +427,16 @@ PageState state_of(const torch::Tensor& table, const torch::Tensor& lens, const 
   for (const auto* t : {&table, &lens, &refs, &table_out, &lens_out, &refs_out}) check_int_vec(*t, op, table);
   TORCH_CHECK(table_out.sizes() == table.sizes() && lens_out.sizes() == lens.sizes() &&
                   refs_out.sizes() == refs.sizes(), op, ": shapes of the outputs");
-  const bool in_place = table_out.data_ptr() == table.data_ptr();
-  TORCH_CHECK(table.numel() == 0 || ((lens_out.data_ptr() == lens.data_ptr()) == in_place &&
-                                     (refs_out.data_ptr() == refs.data_ptr()) == (in_place || refs.numel() == 0)),
-              op, ": table, lens and refs are written all in place or all out of place");
+  // Tensors without entries have no place of their own: they go with the others.
+  int same = 0, other = 0;
+  for (const auto& [in, to] : {std::pair(&table, &table_out), std::pair(&lens, &lens_out), std::pair(&refs, &refs_out)})
+    if (in->numel()) (in->data_ptr() == to->data_ptr() ? same : other)++;
+  TORCH_CHECK(!same || !other, op, ": table, lens and refs are written all in place or all out of place");
   TORCH_CHECK(page >= 1 && table.size(0) <= INT32_MAX / 8 && refs.size(0) <= INT32_MAX / 8 &&
                   table.size(1) * page <= INT32_MAX, op, ": sizes");
   return PageState{table.data_ptr<int>(), lens.data_ptr<int>(), refs.data_ptr<int>(), table_out.data_ptr<int>(),
                    lens_out.data_ptr<int>(), refs_out.data_ptr<int>(), int(table.size(0)), int(table.size(1)),
-                   int(refs.size(0)), int(page), error_word()};
+                   int(refs.size(0)), int(page), other > 0, error_word()};
 }
 
 int* room_of(const c10::optional<torch::Tensor>& room, const torch::Tensor& lens, const char* op) {

@@ -269,3 +269,26 @@ def test_members_shorter_than_the_prefix_do_not_see_its_end():
         ok = ref.isfinite()
         vmax = b.v[torch.isfinite(b.v)].abs().max().item()
         assert (out - ref)[ok].abs().max() <= (2 * 2.0 ** -8 + 4e-4) * vmax
+
+
+# ---- states without entries, rows without a place --------------------------------------------
+
+
+@gpu
+@checked
+@pytest.mark.parametrize("pages,width,slots", [(5, 3, 0), (5, 0, 4), (0, 3, 4), (0, 0, 0)])
+def test_states_without_entries(pages, width, slots):
+    """Fresh outputs are written whole, also where the table has no entries."""
+    from rs_nanogpt_b200.ops import paged
+    table = torch.full((slots, width), -1, device=DEV, dtype=torch.int32)
+    lens, refs = _i32([0] * slots), _i32([0] * pages)
+    none, k = _i32([]), torch.zeros(1, pages, 1, 4, 8, device=DEV)
+    for call in (lambda out: paged.grow_pages(table, lens, refs, _i32([0] * slots), 4, out=out),
+                 lambda out: paged.free_pages(table, lens, refs, none, out=out),
+                 lambda out: paged.fork_pages(k, k.clone(), table, lens, refs, none, none, out=out),
+                 lambda out: paged.compact_pages(k, k.clone(), table, lens, refs, out=out)):
+        out = tuple(torch.full_like(x, 77) for x in (table, lens, refs))
+        call(out)
+        for x, want in zip(out, (table, lens, refs)):
+            assert torch.equal(x, want)
+        assert all(torch.equal(x, want) for x, want in zip(call((table, lens, refs)), (table, lens, refs)))
