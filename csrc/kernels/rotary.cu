@@ -197,21 +197,21 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     va[n] = *reinterpret_cast<const Vec<T, V>*>(src + oa[n]);
     vb[n] = *reinterpret_cast<const Vec<T, V>*>(src + ob[n]);
   }
+  // A row that stands nowhere: 0 in q's output, not what its memory held.
+  auto nowhere = [&](int code) {
+    if (code && lane == 0) atomicCAS(a.err, 0, code);
+    if (!is_q) return;
+    T* dst = static_cast<T*>(t.dst) + row * t.dst_row + i * t.dst_head;
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+      *reinterpret_cast<Vec<T, V>*>(dst + oa[n]) = *reinterpret_cast<Vec<T, V>*>(dst + ob[n]) = Vec<T, V>{};
+  };
   const int slot = a.row_slot[row];
-  if (slot < 0 || slot >= a.slots) {
-    if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
-    return;
-  }
+  if (slot < 0 || slot >= a.slots) return nowhere(kErrBounds);
   const int back = a.row_back[row], p = a.lens[slot] - 1 - back;
-  if (p < 0) return;  // a slot that holds fewer tokens than its rows: nothing to write
-  if (a.room && back >= a.room[slot]) {  // the place of a token that the cache already holds
-    if (lane == 0) atomicCAS(a.err, 0, kErrNoPages);
-    return;
-  }
-  if (p >= a.positions || p >= a.width * a.page) {
-    if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
-    return;
-  }
+  if (p < 0) return nowhere(kErrNone);  // a slot that holds fewer tokens than its rows: nothing to write
+  if (a.room && back >= a.room[slot]) return nowhere(kErrNoPages);  // the place of a token that the cache holds
+  if (p >= a.positions || p >= a.width * a.page) return nowhere(kErrBounds);
   T* dst;
   if (is_q) {
     dst = static_cast<T*>(t.dst) + row * t.dst_row + i * t.dst_head;

@@ -181,8 +181,9 @@ def append(q, k, v, k_pages, v_pages, table, lens, plan: PrefixPlan, cos=None, s
     RoPE (rs-nanogpt src/model/attention.rs:68-116), which takes a factor common
     to ``cos`` and ``sin`` out again (see ``rotary.Scaling``). ``lens`` counts the new
     tokens already (``grow_pages`` comes first); with ``room``, tokens that it
-    did not grant are left out and reported. Returns q, turned and normed
-    alike, in ``q_out`` (which may be q)."""
+    did not grant are left out and reported. Returns q, turned and normed alike,
+    in ``q_out`` (which may be q); rows without a place in the cache, those
+    of an empty slot among them, are 0 there."""
     if q_out is None:
         q_out = torch.empty_like(q)
     ext().paged_append(q, k, v, k_pages, v_pages, table, lens, plan.row_slot, plan.row_back, cos, sin,

@@ -292,3 +292,17 @@ def test_states_without_entries(pages, width, slots):
         for x, want in zip(out, (table, lens, refs)):
             assert torch.equal(x, want)
         assert all(torch.equal(x, want) for x, want in zip(call((table, lens, refs)), (table, lens, refs)))
+
+
+@gpu
+@checked
+def test_rows_without_a_place_are_zero():
+    """The rows of q of a slot that holds no tokens, or fewer than its rows, are 0, not what memory held."""
+    from rs_nanogpt_b200.ops import paged
+    b = Batch([(3, 0)], [5, 6, 9], [2, 6, 4], 4, 2, 64, 32, torch.bfloat16)
+    b.dev_lens = _i32([0, 4, 9])
+    k, v = (torch.randn(12, 2, 64, device=DEV).bfloat16() for _ in range(2))
+    out = torch.full(b.q.shape, 7.0, device=DEV, dtype=torch.bfloat16)
+    q = b.q.to(DEV)
+    paged.append(q, k, v, b.k.to(DEV), b.v.to(DEV), b.dev_table, b.dev_lens, b.plan, q_out=out)
+    assert (out[:4] == 0).all() and torch.equal(out[4:], q[4:])
