@@ -15,7 +15,8 @@ import functools
 _LAUNCHES = {"flash_bwd": 3, "flash_bwd_tc": lambda *a, **k: 2 if (a[-1] is True or k.get("prepared")) else 3,
              "flash_bwd_prep": 1, "kernel_status": 0, "flash_fwd_tc_supported": 0,
              "flash_bwd_tc_supported": 0, "flash_bwd_trace": 0, "gemm_trace": 0, "set_pdl": 0,
-             "pages_fork": 2, "pages_compact": 2, "paged_attention": 2,
+             "pages_fork": 2, "pages_compact": 2,
+             "paged_attention": 0,  # its plan knows (ops/paged.py)
              "decode_attention": lambda qkv, kc, vc, pos, out, po, pm, chunk: 1 + int(kc.shape[2] > chunk)}
 _count = [0]
 
@@ -48,6 +49,11 @@ def ext():
 
 def launch_count() -> int:
     return _count[0]
+
+
+def count_launches(n: int) -> None:
+    """For calls whose number of kernels their caller knows."""
+    _count[0] += n
 
 
 def kernel_status(reset: bool = True) -> int:

@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from . import rotary
-from ._ext import ext
+from ._ext import count_launches, ext
 
 State = Tuple[torch.Tensor, torch.Tensor, torch.Tensor]
 
@@ -166,6 +166,8 @@ class PrefixPlan:
         def dev(x):
             return torch.as_tensor(np.ascontiguousarray(x), dtype=torch.int32).to(device)
 
+        kinds = sum(1 for x in lists if x)
+        self.launches = kinds + (kinds > 0)  # of an attention call: a kernel for either kind of items, and the join
         self.items, self.big_items = (dev(np.asarray(x, np.int64).reshape(-1, 8)) for x in lists)
         self.shared_item, self.own_item = dev(of_pair[1]), dev(of_pair[0])
         self.slot_of_seq, self.row_slot, self.row_back = dev(slot), dev(slot[seq]), dev(back)
@@ -206,4 +208,5 @@ def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[
     ext().paged_attention(q, k_pages, v_pages, table, lens, plan.items, plan.big_items, plan.slot_of_seq, plan.row_slot,
                           plan.row_back, plan.shared_item, plan.own_item, plan.max_slot, plan.page,
                           q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
+    count_launches(plan.launches)
     return out
