@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from test_paged import DEV, Batch, Model, _check_state, _i32, _pools, _state
+from test_paged import CASES, DEV, Batch, Model, _check_state, _i32, _pools, _state
 
 gpu = pytest.mark.gpu
 checked = pytest.mark.usefixtures("kernel_ok")
@@ -306,3 +306,38 @@ def test_rows_without_a_place_are_zero():
     q = b.q.to(DEV)
     paged.append(q, k, v, b.k.to(DEV), b.v.to(DEV), b.dev_table, b.dev_lens, b.plan, q_out=out)
     assert (out[:4] == 0).all() and torch.equal(out[4:], q[4:])
+
+
+# ---- how near the attention comes ------------------------------------------------------------
+
+
+@gpu
+@checked
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", CASES)
+def test_attention_error_scales_with_the_probabilities(name, dtype):
+    """Rounding each p_j to the type (relative error up to u) moves an output by a sum of terms u p_j v_j of
+    either sign: by more than 7 u sqrt(sum (p_j v_j)^2) in one element of 2e10 (Hoeffding). fp16 loses up to
+    2^-25 of the largest p on small ones. The output is rounded once, by u |o|. Scores, exponentials and sums
+    in fp32: scores are off by less than 2e-4, which counts twice, and sums by less than 1e-4, both times
+    sum p_j |v_j|. An output of zeros is far outside of this, also behind a prefix of 20000 tokens."""
+    b = Batch(*CASES[name], dtype)
+    out = b.run().double()
+    unit = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    row = 0
+    for s in range(b.n):
+        n, t = b.lens[s], b.q_lens[s]
+        ids = b.table[s, :-(-n // b.page)].long()
+        k, v = (x[ids].transpose(0, 1).flatten(1, 2)[:, :n].to(DEV).double().repeat_interleave(b.hq // b.hk, 0)
+                for x in (b.k, b.v))
+        z = torch.einsum("thd,hnd->htn", b.q[row:row + t].to(DEV).double(), k) / math.sqrt(b.d)
+        z.masked_fill_(torch.ones(t, n, device=DEV, dtype=torch.bool).triu(n - t + 1), -math.inf)
+        p = torch.softmax(z, -1)
+        ref, mass = p @ v, p @ v.abs()
+        tol = 7 * unit * (p.square() @ v.square()).sqrt() + unit * ref.abs() + 5e-4 * mass
+        if dtype == torch.float16:
+            tol += 2.0 ** -25 * p.amax(-1, keepdim=True) * v.abs().sum(1, keepdim=True)
+        got = out[row:row + t].transpose(0, 1)
+        assert ((got - ref).abs() <= tol).all(), ((got - ref).abs() / tol).max().item()
+        assert (ref.abs() > tol).any(-1).all()
+        row += t
