@@ -78,7 +78,8 @@ void pages_copy(torch::Tensor k, torch::Tensor v, torch::Tensor src, torch::Tens
 void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                      torch::Tensor items, torch::Tensor big_items, torch::Tensor slot_of_seq, torch::Tensor row_slot,
                      torch::Tensor row_back, torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot,
-                     int64_t plan_page, double scale, torch::Tensor out, c10::optional<torch::Tensor> lse);
+                     int64_t plan_page, int64_t plan_keys, double scale, torch::Tensor out,
+                     c10::optional<torch::Tensor> lse);
 torch::Tensor gemm_trace();
 }  // namespace nk
 

@@ -28,7 +28,9 @@ struct Lattice {
   int64_t run() const { return (inner - 1) * inner_stride + item; }
   int64_t end() const { return at + (outer - 1) * outer_stride + run(); }
   // No byte of it is named twice.
-  bool simple() const { return empty || ((inner == 1 || inner_stride >= item) && (outer == 1 || outer_stride >= run())); }
+  bool simple() const {
+    return empty || ((inner == 1 || inner_stride >= item) && (outer == 1 || outer_stride >= run()));
+  }
 };
 
 // Two runs of m and n bytes, `gap` apart, that both repeat every `period` bytes.

@@ -30,6 +30,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <climits>
 
 #include "flash_common.cuh"
@@ -602,11 +603,13 @@ void launch(const torch::Tensor& k, const torch::Tensor& v, const Args& a, const
 // q, out: (rows, query heads, head_dim); k, v: one layer's pages (pages, kv heads,
 // rows of a page, head_dim). items, big_items: (n, 8) int32; shared_item, own_item:
 // item of each (row, query head of a kv head), plus kBig for big items, -1 where
-// there is none. plan_page: rows of the pages that the items were made for.
+// there is none. plan_page: rows of the pages that the items were made for;
+// plan_keys: keys of the longest shared run.
 void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor table, torch::Tensor lens,
                      torch::Tensor items, torch::Tensor big_items, torch::Tensor slot_of_seq, torch::Tensor row_slot,
                      torch::Tensor row_back, torch::Tensor shared_item, torch::Tensor own_item, int64_t max_slot,
-                     int64_t plan_page, double scale, torch::Tensor out, c10::optional<torch::Tensor> lse) {
+                     int64_t plan_page, int64_t plan_keys, double scale, torch::Tensor out,
+                     c10::optional<torch::Tensor> lse) {
   using namespace pa;
   const auto type = q.scalar_type();
   TORCH_CHECK(q.is_cuda(), "paged_attention: q must be on a GPU");
@@ -647,8 +650,11 @@ void paged_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   TORCH_CHECK(shared_item.numel() == rows * share, "paged_attention: the plan is for ",
               num(rows ? shared_item.numel() / rows : 0), " query heads a kv head, q has ", num(share));
   TORCH_CHECK(scale > 0, "paged_attention: scale must be positive");
-  TORCH_CHECK(rows * hq <= (int64_t(1) << 28) && table.size(1) * page <= INT32_MAX &&
-                  (items.size(0) + big_items.size(0)) * hk * (4 + table.size(1) * page / 32) <= INT32_MAX,
+  // A shared run is as long as the plan says, whatever the table holds. The room below
+  // the limit is for the last worker's share, which may end past the last unit.
+  const int64_t most_keys = std::max(table.size(1) * page, plan_keys);
+  TORCH_CHECK(rows * hq <= (int64_t(1) << 28) && most_keys <= INT32_MAX &&
+                  (items.size(0) + big_items.size(0)) * hk * (4 + most_keys / 32) <= INT32_MAX - (1 << 16),
               "paged_attention: more rows or tiles than 32-bit numbers count");
   if (lse.has_value()) {
     TORCH_CHECK(lse->device() == q.device() && lse->scalar_type() == at::kFloat && lse->is_contiguous() &&

@@ -128,6 +128,7 @@ class PrefixPlan:
             raise ValueError(f"slots must be one table row for each of the {n_seq} sequences")
         share = n_head // n_kv_head
         self.rows, self.share, self.max_slot = int(t.sum()), share, int(slot.max(initial=-1))
+        self.max_shared = max((s for _, s in groups), default=0)
         self.n_head, self.n_kv_head, self.head_dim, self.page, self.table_width = (n_head, n_kv_head, head_dim, page,
                                                                                    table_width)
         start = np.concatenate([[0], np.cumsum(t)])
@@ -207,6 +208,6 @@ def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[
         out = torch.empty_like(q)
     ext().paged_attention(q, k_pages, v_pages, table, lens, plan.items, plan.big_items, plan.slot_of_seq, plan.row_slot,
                           plan.row_back, plan.shared_item, plan.own_item, plan.max_slot, plan.page,
-                          q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
+                          plan.max_shared, q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
     count_launches(plan.launches)
     return out

@@ -158,6 +158,18 @@ def test_a_plan_for_other_pages_is_refused():
 
 @gpu
 @checked
+def test_more_tiles_than_are_counted_are_refused():
+    """The limit counts the keys of the plan's shared runs, not only those that the table at hand can name."""
+    from rs_nanogpt_b200.ops import paged
+    b = Batch([(30, 64)], [5] * 30, 1, 4, 2, 64, 32, torch.bfloat16)
+    b.plan = paged.PrefixPlan([(30, 1 << 30)], 1, n_head=4, n_kv_head=2, head_dim=64, page=32, table_width=1 << 25)
+    assert len(b.plan.items) + len(b.plan.big_items) > 30  # the shared run is one of its own
+    with pytest.raises(RuntimeError, match="32-bit"):
+        b.run()
+
+
+@gpu
+@checked
 def test_outputs_over_other_operands_are_refused():
     from rs_nanogpt_b200.ops import paged, rotary
     n, h, d = 6, 2, 64
