@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   const bool is_q = h < a.hq, is_v = h >= a.hq + a.hk;
   const Heads& t = is_q ? a.q : (is_v ? a.v : a.k);
   const int i = is_q ? h : (is_v ? h - a.hq - a.hk : h - a.hq);
+  const int slot = __ldg(a.row_slot + row), back = __ldg(a.row_back + row);
   // The values are on their way while the row's place is looked up.
   const T* src = static_cast<const T*>(t.src) + row * t.src_row + i * t.src_head;
   Vec<T, V> va[NI], vb[NI];
@@ -206,9 +207,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     for (int n = 0; n < NI; ++n)
       *reinterpret_cast<Vec<T, V>*>(dst + oa[n]) = *reinterpret_cast<Vec<T, V>*>(dst + ob[n]) = Vec<T, V>{};
   };
-  const int slot = a.row_slot[row];
   if (slot < 0 || slot >= a.slots) return nowhere(kErrBounds);
-  const int back = a.row_back[row], p = a.lens[slot] - 1 - back;
+  const int p = __ldg(a.lens + slot) - 1 - back;
   if (p < 0) return nowhere(kErrNone);  // a slot that holds fewer tokens than its rows: nothing to write
   if (a.room && back >= a.room[slot]) return nowhere(kErrNoPages);  // the place of a token that the cache holds
   if (p >= a.positions || p >= a.width * a.page) return nowhere(kErrBounds);
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   if (is_q) {
     dst = static_cast<T*>(t.dst) + row * t.dst_row + i * t.dst_head;
   } else {
-    const int page = a.table[long(slot) * a.width + p / a.page];
+    const int page = __ldg(a.table + long(slot) * a.width + p / a.page);
     if (page < 0 || page >= a.pages) {
       if (lane == 0) atomicCAS(a.err, 0, kErrBounds);
       return;
