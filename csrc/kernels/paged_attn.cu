@@ -429,10 +429,12 @@ __device__ __noinline__ void attend_alone(const Args& a, const int* shared_item,
 // where there are few pairs and so many partials of each (latency counts), eight
 // where there are many pairs of few partials (loads in flight count).
 constexpr int kJoinThreads = 128;
-// The CTAs an SM keep the registers at what the join itself needs: attend_alone, which
-// hardly any call reaches, may spill.
+// With eight lanes a pair there are many CTAs, and the registers are held at what the
+// join itself needs (attend_alone, which hardly any call reaches, may spill): 99 us
+// instead of 101 for a call of 33 prompts. With 32 there are few, and the bound would
+// cost 1 us of 15.
 template <typename T, int D, int L>
-__global__ void __launch_bounds__(kJoinThreads, D == 128 && L == 8 ? 7 : 9)
+__global__ void __launch_bounds__(kJoinThreads, L == 32 ? 1 : (D == 128 ? 7 : 9))
     paged_join_kernel(const __grid_constant__ Args a, const int* __restrict__ shared_item,
                       const int* __restrict__ own_item) {
   constexpr int E = D / L, U = 4 * L / 32 + 1, W = E < 4 ? E : 4;  // W: floats of a load
