@@ -17,7 +17,8 @@
 //               only when a row's maximum grew by 2^8 or more since the last time; the
 //               stale maximum scales P and O alike.
 // Keys past the end of an item's run are hidden by the mask; their values are
-// cleared in shared memory first, since 0 * NaN is not 0.
+// cleared in shared memory first, since 0 * NaN is not 0. Rows that a NaN of a key
+// which only other rows see has reached are done again by the join (paged_attn.cu).
 //
 // Measured (one B200): 1024 rows against 32768 keys on 4 kv heads of 128 (69 GFLOP) in
 // 81 us, 849 TFLOP/s; a tile of 256 rows and 128 keys takes about 3600 cycles, of which

@@ -10,7 +10,9 @@ which is prefilled, stored and, in every decode step, read once for all of them.
 The decoder's positions may go past the trained ``sequence_len`` with a
 ``rotary.Scaling``. Its sums are the cached forward's of ``models/decode.py``
 (rs-nanogpt src/model/gpt.rs:80-131) except that the divisor of the q/k norm is
-kept in fp32 instead of being rounded to bf16 first.
+kept in fp32 instead of being rounded to bf16 first, and that the softmax's
+probabilities are rounded to bf16 before they meet the values, as in the
+training forward; the decode step there keeps them in fp32.
 """
 from typing import List, Optional, Sequence, Tuple
 

@@ -109,7 +109,10 @@ class PrefixPlan:
     all, or a list); the rows of q, k and v hold them one sequence after another.
     ``slots`` names each sequence's row of the cache's table (0, 1, 2, ... by
     default). A plan depends on nothing that changes from step to step, so one
-    plan serves every layer and every step of a batch, and a captured graph."""
+    plan serves every layer and every step of a batch, and a captured graph.
+    Making one takes the host 0.3 ms for a few sequences to 0.8 ms for 256 (lists
+    in Python, eight copies to the device), more than the attention of one layer:
+    it is meant to be kept."""
 
     def __init__(self, groups: Sequence[Tuple[int, int]], q_lens: Union[int, Sequence[int]] = 1, *, n_head: int,
                  n_kv_head: int, head_dim: int, page: int, table_width: int, slots: Optional[Sequence[int]] = None,
@@ -201,7 +204,8 @@ def attention(q, k_pages, v_pages, table, lens, plan: PrefixPlan, out: Optional[
     layer's pages, the keys that a group shares read once for all its rows.
     ``lens`` counts the new tokens; the last of them sees all of its sequence. A
     row without keys (an empty slot) gives 0. A NaN or infinite value reaches
-    the rows that see its key and no others. ``out`` may be q. ``lse`` (rows, heads) fp32 takes
+    the rows that see its key and no others. The probabilities are rounded to
+    the values' type before they meet them, their sum is not. ``out`` may be q. ``lse`` (rows, heads) fp32 takes
     the log of each row's softmax sum (-inf without keys). ``scale`` is
     1 / sqrt(head_dim) by default."""
     if out is None:
